@@ -138,11 +138,15 @@ int psi_hip_ctx_set_flag(psi_hip_ctx* ctx, uint32_t flag, uint32_t value);
  *                 |v| > 65504, Inf or NaN): that map multiplies V as f16.  Run the batch through
  *                 psi_hip_split_kv_tiled_q_map instead, which keeps V in the storage type -- except for tiles of
  *                 more than 48 query columns, which that entry point hands to the same kernel: for those, set
- *                 PSI_HIP_FLAG_FORCE_GENERIC for the step (the shape-generic kernels multiply in f32).
+ *                 PSI_HIP_FLAG_FORCE_GENERIC for the step (the shape-generic kernels multiply in f32);
+ *   CACHE_RANGE   an operator of the section "cache eviction" met a request slot, position or page ID outside the
+ *                 bounds it was given (the page table, the arena, the accumulators, max_context_tokens, a table of
+ *                 kept positions that does not ascend): what it names was left out and stays as it was.
  * psi_hip_sync returns PSI_HIP_ERR_RUNTIME while a bit is set; psi_hip_ctx_take_device_error
  * synchronises the context's stream, returns the bits and clears them. */
 #define PSI_HIP_DEVICE_ERR_WAIT_GAVE_UP 1u
 #define PSI_HIP_DEVICE_ERR_V_RANGE 2u
+#define PSI_HIP_DEVICE_ERR_CACHE_RANGE 4u
 int psi_hip_ctx_take_device_error(psi_hip_ctx* ctx, uint32_t* out_bits);
 
 /* Device-side active counts for captured launches: the counterpart of `ReplayU32::Parameter`
@@ -791,6 +795,109 @@ int psi_hip_gqa_replay_cache_submit(psi_hip_gqa_replay_cache* cache, const psi_h
 /* Programs held, recordings and replays so far; any out pointer may be null. */
 int psi_hip_gqa_replay_cache_stats(const psi_hip_gqa_replay_cache* cache, uint32_t* programs, uint64_t* recordings,
                                    uint64_t* replays);
+
+/* ------------------------------------------------------------------ cache eviction
+ *
+ * Bounds what a long sequence's cache costs: of each request and KV head only the tokens that the attention has used
+ * most are kept.  No counterpart in the reference, whose caches grow with their sequences.  Four operators:
+ *   attend_weights   the decode attention, which also adds to every cached token the attention weight it received;
+ *   observe_weights  the same weights for the last tokens of a prompt (no attention output): what a prompt is cut by;
+ *   select_kept      the positions to keep: the first num_first, the last num_recent, then the heaviest;
+ *   compact          moves the kept lines and accumulators to the front of the request's pages.
+ * Afterwards a request holds `budget` cached tokens: pages behind them can go back to the allocator, its next token is
+ * appended at position `budget` (token_index of the next step), and the attention entry points above serve it as they
+ * are.  Keys stay rotated for the positions they were written at, so the rotary position of a new token counts on
+ * (psi_hip_rms_norm_rope with positions of its own, then the split-row form of the layer); the layer's fused
+ * projection form, which takes the cache position for the rotary position, is for requests that were never compacted.
+ *
+ * Accumulators: page_weights, device f32 [page][num_kv_heads][tokens_per_page], found through the same page IDs as K
+ * and V (every layer's pages are its own, so one array serves all layers).  A step starts the accumulators of the
+ * tokens it appends from zero, so a page taken from the allocator needs no clearing.  A page belongs to one request;
+ * page IDs beyond the arena or the accumulators are left out (PSI_HIP_DEVICE_ERR_CACHE_RANGE).
+ * Weights, normalisers and sums are f32 whatever the cache's type.  Nothing is added atomically: the same call gives
+ * the same bits on every run.  These entry points allocate nothing and can be captured into a graph; two launches of
+ * one scratch, logits or kept buffer must follow one another. */
+
+/* Bytes of page_weights for an arena of num_pages pages. */
+int psi_hip_kv_page_weights_bytes(const psi_hip_gqa_config* cfg, uint64_t num_pages, uint64_t* out_bytes);
+
+typedef struct psi_hip_kv_weights {
+    float* page_weights;
+    uint64_t page_weights_bytes;
+    void* logits; /* device scratch of psi_hip_split_kv_single_q_logits_bytes, 16-byte aligned */
+    uint64_t logits_bytes;
+    uint32_t max_context_tokens; /* bound on the context of any token of the step; keys beyond it are attended, but
+                                    their accumulators stay as they were (PSI_HIP_DEVICE_ERR_CACHE_RANGE) */
+    float decay;                 /* 0 .. 1: what earlier steps' weights are multiplied by, 1 = plain sums */
+} psi_hip_kv_weights;
+
+/* Bytes of the logits that a step of up to num_total_tokens tokens stores, [tokens][num_q_heads][max_context_tokens
+ * rounded up to 16] f32. */
+int psi_hip_split_kv_single_q_logits_bytes(const psi_hip_gqa_config* cfg, uint32_t num_total_tokens,
+                                           uint32_t max_context_tokens, uint64_t* out_bytes);
+
+/* A decode step's attention (append if flat_k / flat_v are set, map, combine with optional gate: the calls above, same
+ * arguments and results) that also accumulates the attention weights of its tokens:
+ *   acc[h][p] = (p < position of the request's first token of this step ? decay * acc[h][p] : 0)
+ *               + sum over the request's tokens t of this step with p <= position(t), and over the query heads g of KV
+ *                 head h, of softmax_p(scale * q[t][g] . k[h][p])
+ * for every position p of the context.  The tokens of a request are adjacent and in position order, and the rows of
+ * its last token tile [0, position + 1) (true of every plan of psi_hip_gqa_metadata_update, also balanced or
+ * re-ordered).  Every row is this step's own: no slots for a second producer.  Honours bound replay counts. */
+int psi_hip_split_kv_single_q_attend_weights(
+    psi_hip_ctx* ctx, const psi_hip_gqa_config* cfg, const psi_hip_page_table_layout* layout, const void* q,
+    void* kv_pages, uint64_t kv_pages_bytes, const void* flat_k, const void* flat_v, const uint32_t* req_slots,
+    const uint32_t* flat_token_indices, const uint32_t* page_ids, const uint32_t* kv_splits,
+    const uint32_t* cu_kv_splits, const uint32_t* worker_cu, uint32_t num_workers, const uint32_t* partial_row_index,
+    void* scratch, uint64_t scratch_bytes, void* output, const psi_hip_output_gate* gate,
+    const psi_hip_kv_weights* weights, uint32_t gqa_layer_index, uint32_t num_total_tokens,
+    uint32_t num_total_kv_splits, uint32_t num_active_tokens, uint32_t num_active_kv_splits);
+
+/* Host plan of an observation: request r brings query tokens cu_tokens[r] .. cu_tokens[r + 1] (at least one) at positions
+ * token_indices[r] ..; its keys are the cached positions up to each token's own.  num_held[r]: the positions whose
+ * accumulators count already, the others start from zero (null: token_indices, as in a decode step; 0 for a prompt's
+ * first observation).  A slot may be named once.  windows: host u32[num_reqs][8], rows: host u32[rows_capacity][3]; both
+ * null to query the out values only.  512 + num_reqs rows always suffice. */
+int psi_hip_kv_observe_plan(const psi_hip_gqa_config* cfg, const psi_hip_page_table_layout* layout,
+                            const uint32_t* req_slots, const uint32_t* token_indices, const uint32_t* cu_tokens,
+                            const uint32_t* num_held, uint32_t num_reqs, uint32_t* windows, uint32_t* rows,
+                            uint32_t rows_capacity, uint32_t* out_num_rows, uint32_t* out_max_window,
+                            uint64_t* out_scratch_bytes);
+
+/* Adds the weights of the planned windows to the accumulators (the formula above with p < num_held in place of the
+ * step's first position; K only).  q: device [num_q_tokens][num_q_heads][head_dim] in the cache's type, normalised and
+ * rotated; windows, rows: device copies of the plan's tables; scratch: the plan's out_scratch_bytes.  The keys of the
+ * query tokens themselves have to be in the cache.  Not while device-side counts are bound. */
+int psi_hip_kv_observe_weights(psi_hip_ctx* ctx, const psi_hip_gqa_config* cfg, const psi_hip_page_table_layout* layout,
+                               const void* q, uint32_t num_q_tokens, const void* kv_pages, uint64_t kv_pages_bytes,
+                               const uint32_t* page_ids, const uint32_t* windows, uint32_t num_windows,
+                               uint32_t max_window, const uint32_t* rows, uint32_t num_rows, void* scratch,
+                               uint64_t scratch_bytes, float* page_weights, uint64_t page_weights_bytes, float decay,
+                               uint32_t gqa_layer_index);
+
+/* Host plan of an eviction: request r holds num_cached[r] tokens (0 is allowed).  A slot may be named once.  requests:
+ * host u32[num_reqs][2], to be copied to the device for the two calls below; *out_max_cached: the longest. */
+int psi_hip_kv_evict_plan(const psi_hip_gqa_config* cfg, const psi_hip_page_table_layout* layout,
+                          const uint32_t* req_slots, const uint32_t* num_cached, uint32_t num_reqs, uint32_t* requests,
+                          uint32_t* out_max_cached);
+
+/* kept: device u32[num_reqs][num_kv_heads][budget], the positions to keep in ascending order, padded with
+ * PSI_HIP_SENTINEL: all of a request of up to `budget` tokens; of a longer one the first num_first, the last num_recent
+ * (together at most budget) and the heaviest of the others, of equal weights the lower position.  NaN counts as -inf.
+ * max_cached_tokens: the plan's.  Not while device-side counts are bound. */
+int psi_hip_kv_select_kept(psi_hip_ctx* ctx, const psi_hip_gqa_config* cfg, const psi_hip_page_table_layout* layout,
+                           const float* page_weights, uint64_t page_weights_bytes, const uint32_t* page_ids,
+                           const uint32_t* requests, uint32_t num_reqs, uint32_t max_cached_tokens, uint32_t budget,
+                           uint32_t num_first, uint32_t num_recent, uint32_t* kept, uint32_t gqa_layer_index);
+
+/* Moves the K and V lines, and the accumulators unless page_weights is null, of position kept[i] to position i, in
+ * place, for every request of more than `budget` tokens.  The kept positions of a (request, head) ascend, as the
+ * selection writes them; an entry that lies outside the cached tokens or below its own index moves nothing.  Positions
+ * from `budget` on keep their bytes.  Not while device-side counts are bound. */
+int psi_hip_kv_compact(psi_hip_ctx* ctx, const psi_hip_gqa_config* cfg, const psi_hip_page_table_layout* layout,
+                       void* kv_pages, uint64_t kv_pages_bytes, float* page_weights, uint64_t page_weights_bytes,
+                       const uint32_t* page_ids, const uint32_t* requests, uint32_t num_reqs,
+                       uint32_t max_cached_tokens, uint32_t budget, const uint32_t* kept, uint32_t gqa_layer_index);
 
 /* ------------------------------------------------------------------ request page table */
 

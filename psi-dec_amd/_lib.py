@@ -25,6 +25,7 @@ FLAG_F32_OUTPUT = 2
 FLAG_MUTE_LOADERS = 3
 DEVICE_ERR_WAIT_GAVE_UP = 1
 DEVICE_ERR_V_RANGE = 2
+DEVICE_ERR_CACHE_RANGE = 4
 REPLAY_EXACT, REPLAY_BUCKETED = 0, 1
 DISPATCH_PLAN_ORDER, DISPATCH_LONGEST_FIRST, DISPATCH_BALANCED, DISPATCH_ROW_GROUPS, DISPATCH_AUTO = 0, 1, 2, 3, 4
 STATIC_SCRATCH_BYTES = 16 << 20
@@ -90,6 +91,17 @@ class RMSNormRopeConfigStruct(ctypes.Structure):
         ("rope_theta", c_float),
         ("scaling", RopeScalingStruct),
         ("dtype", c_uint32),
+    ]
+
+
+class KVWeightsStruct(ctypes.Structure):
+    _fields_ = [
+        ("page_weights", c_void_p),
+        ("page_weights_bytes", c_uint64),
+        ("logits", c_void_p),
+        ("logits_bytes", c_uint64),
+        ("max_context_tokens", c_uint32),
+        ("decay", c_float),
     ]
 
 
@@ -375,6 +387,25 @@ PROTOTYPES = {
     "psi_hip_gqa_replay_cache_destroy": (c_int, [c_void_p]),
     "psi_hip_gqa_replay_cache_submit": (c_int, [c_void_p, POINTER(LayerInputStruct), c_uint32, POINTER(c_int)]),
     "psi_hip_gqa_replay_cache_stats": (c_int, [c_void_p, _U32P, _U64P, _U64P]),
+    "psi_hip_kv_page_weights_bytes": (c_int, [_CFG, c_uint64, POINTER(c_uint64)]),
+    "psi_hip_split_kv_single_q_logits_bytes": (c_int, [_CFG, c_uint32, c_uint32, POINTER(c_uint64)]),
+    "psi_hip_split_kv_single_q_attend_weights": (
+        c_int, [c_void_p, _CFG, _LAYOUT, c_void_p, c_void_p, c_uint64, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
+                c_void_p, c_void_p, c_void_p, c_uint32, c_void_p, c_void_p, c_uint64, c_void_p,
+                POINTER(OutputGateStruct), POINTER(KVWeightsStruct), c_uint32, c_uint32, c_uint32, c_uint32, c_uint32]),
+    "psi_hip_kv_observe_plan": (
+        c_int, [_CFG, _LAYOUT, _U32P, _U32P, _U32P, _U32P, c_uint32, _U32P, _U32P, c_uint32, _U32P, _U32P,
+                POINTER(c_uint64)]),
+    "psi_hip_kv_observe_weights": (
+        c_int, [c_void_p, _CFG, _LAYOUT, c_void_p, c_uint32, c_void_p, c_uint64, c_void_p, c_void_p, c_uint32, c_uint32,
+                c_void_p, c_uint32, c_void_p, c_uint64, c_void_p, c_uint64, c_float, c_uint32]),
+    "psi_hip_kv_evict_plan": (c_int, [_CFG, _LAYOUT, _U32P, _U32P, c_uint32, _U32P, _U32P]),
+    "psi_hip_kv_select_kept": (
+        c_int, [c_void_p, _CFG, _LAYOUT, c_void_p, c_uint64, c_void_p, c_void_p, c_uint32, c_uint32, c_uint32, c_uint32,
+                c_uint32, c_void_p, c_uint32]),
+    "psi_hip_kv_compact": (
+        c_int, [c_void_p, _CFG, _LAYOUT, c_void_p, c_uint64, c_void_p, c_uint64, c_void_p, c_void_p, c_uint32, c_uint32,
+                c_uint32, c_void_p, c_uint32]),
     "psi_hip_page_table_write_page_ids": (
         c_int, [c_void_p, _LAYOUT, c_void_p, c_uint32, c_uint32, c_uint32, _U32P, c_uint32, c_uint32]),
     "psi_hip_page_table_reset_req_slot": (c_int, [c_void_p, _LAYOUT, c_void_p, c_uint32]),

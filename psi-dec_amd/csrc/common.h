@@ -45,7 +45,7 @@ int make_geometry(const psi_hip_gqa_config* cfg, Geometry* g);
 int resolve_static_scratch(int device);
 int check_layout(const psi_hip_page_table_layout* layout);
 
-constexpr uint32_t kDeviceStatusWords = 2;
+constexpr uint32_t kDeviceStatusWords = 3;
 constexpr uint32_t kDefaultWaitPolls = 1u << 16;
 
 struct KernelTimer {

@@ -177,9 +177,10 @@ static uint32_t device_error_bits(const psi_hip_ctx* ctx) {
 
 static int report_device_error(uint32_t bits) {
     if (bits == 0) return PSI_HIP_OK;
-    return psi::fail(PSI_HIP_ERR_RUNTIME, "a kernel reported an error (bits 0x%x):%s%s; the affected partial rows are empty states",
+    return psi::fail(PSI_HIP_ERR_RUNTIME, "a kernel reported an error (bits 0x%x):%s%s%s; the affected rows are empty states or left as they were",
                      bits, (bits & PSI_HIP_DEVICE_ERR_WAIT_GAVE_UP) ? " a bounded wait between waves ran out" : "",
-                     (bits & PSI_HIP_DEVICE_ERR_V_RANGE) ? " the prefill-chunk map met V values outside the f16 range" : "");
+                     (bits & PSI_HIP_DEVICE_ERR_V_RANGE) ? " the prefill-chunk map met V values outside the f16 range" : "",
+                     (bits & PSI_HIP_DEVICE_ERR_CACHE_RANGE) ? " a cache-eviction operator met a position or page ID outside its bounds" : "");
 }
 
 int psi_hip_sync(psi_hip_ctx* ctx) {

@@ -66,6 +66,10 @@ struct MapArgs {
     uint32_t mute_loaders = 0;
     // Prefill-chunk map: the context's two work-sharing words (psi_hip_ctx::work_claim).
     uint32_t* work_claim = nullptr;
+    // SingleQ map of the attention that accumulates weights (null otherwise): every visible key's logit in the log2
+    // domain goes to logits[(token * hq + q_head) * logits_stride + position], positions below logits_stride only.
+    float* logits = nullptr;
+    uint64_t logits_stride = 0;
 };
 
 // Fills the three fields above from the context.
@@ -177,6 +181,17 @@ inline bool chunk_map_supported(const Geometry& g, uint32_t q_token_tile_size) {
 void launch_map_generic(psi_hip_ctx* ctx, const Geometry& g, const MapArgs& a);
 void launch_reduce_generic(psi_hip_ctx* ctx, const Geometry& g, const ReduceArgs& a, uint32_t num_total_tokens);
 void fill_walk(PageWalk* walk, const Geometry& g, const psi_hip_page_table_layout* layout, const uint32_t* page_ids);
+
+// The SingleQ map behind its public entry points.  flat_k / flat_v / flat_token_indices: null, or the append folded in;
+// logits: null, or where the logits go as well (MapArgs::logits).
+int single_q_map_impl(psi_hip_ctx* ctx, const psi_hip_gqa_config* cfg, const psi_hip_page_table_layout* layout,
+                      const void* q, const void* kv_pages, uint64_t kv_pages_bytes, const uint32_t* req_slots,
+                      const uint32_t* page_ids, const uint32_t* kv_splits, const uint32_t* worker_cu,
+                      uint32_t num_workers, void* scratch, uint64_t scratch_bytes, uint32_t gqa_layer_index,
+                      uint32_t num_total_tokens, uint32_t num_total_kv_splits, uint32_t num_active_tokens,
+                      uint32_t num_active_kv_splits, const void* flat_k = nullptr, const void* flat_v = nullptr,
+                      const uint32_t* flat_token_indices = nullptr, float* logits = nullptr,
+                      uint64_t logits_stride = 0);
 
 // Fast decode map for head_dim 256 / 128, 2-byte elements, power-of-two pages; returns
 // PSI_HIP_ERR_UNSUPPORTED when the shape is outside its domain (caller falls back).

@@ -8,6 +8,11 @@ int launch_decode_map_bf16_d256(psi_hip_ctx* ctx, const Geometry& g, const MapAr
 int launch_decode_map_bf16_d128(psi_hip_ctx* ctx, const Geometry& g, const MapArgs& a);
 int launch_decode_map_f16_d256(psi_hip_ctx* ctx, const Geometry& g, const MapArgs& a);
 int launch_decode_map_f16_d128(psi_hip_ctx* ctx, const Geometry& g, const MapArgs& a);
+// the variants that store the logits as well (MapArgs::logits)
+int launch_decode_logits_bf16_d256(psi_hip_ctx* ctx, const Geometry& g, const MapArgs& a);
+int launch_decode_logits_bf16_d128(psi_hip_ctx* ctx, const Geometry& g, const MapArgs& a);
+int launch_decode_logits_f16_d256(psi_hip_ctx* ctx, const Geometry& g, const MapArgs& a);
+int launch_decode_logits_f16_d128(psi_hip_ctx* ctx, const Geometry& g, const MapArgs& a);
 
 // Log-sum-exp combine: one wave per (token, q_head), lanes over head_dim.  The accumulator rows are
 // read four at a time so that a wave keeps several 1 KiB reads in flight instead of one; the overall
@@ -230,6 +235,11 @@ int launch_decode_map_fast(psi_hip_ctx* ctx, const Geometry& g, const MapArgs& a
     const bool aligned = reinterpret_cast<uintptr_t>(a.q) % 16 == 0 && reinterpret_cast<uintptr_t>(a.kv_pages) % 16 == 0;
     if (!two_byte || !page_ok || !aligned || g.group > 8 || (g.d != 256 && g.d != 128)) return PSI_HIP_ERR_UNSUPPORTED;
     if ((uint64_t)a.num_total_kv_splits * g.hkv > 0x7fffffffull) return PSI_HIP_ERR_UNSUPPORTED;
+    if (a.logits != nullptr) {
+        if (g.dtype == PSI_HIP_BF16)
+            return g.d == 256 ? launch_decode_logits_bf16_d256(ctx, g, a) : launch_decode_logits_bf16_d128(ctx, g, a);
+        return g.d == 256 ? launch_decode_logits_f16_d256(ctx, g, a) : launch_decode_logits_f16_d128(ctx, g, a);
+    }
     if (g.dtype == PSI_HIP_BF16)
         return g.d == 256 ? launch_decode_map_bf16_d256(ctx, g, a) : launch_decode_map_bf16_d128(ctx, g, a);
     return g.d == 256 ? launch_decode_map_f16_d256(ctx, g, a) : launch_decode_map_f16_d128(ctx, g, a);

@@ -107,7 +107,8 @@ struct TilePages {
     uint32_t a, b;
 };
 
-template <typename Tag, int D, int G, int kWaves, bool kHalfPage>
+// kLogits: the logits are stored as well (MapArgs::logits), a variant of its own so that the plain map keeps its code.
+template <typename Tag, int D, int G, int kWaves, bool kHalfPage, bool kLogits = false>
 __global__ __launch_bounds__(64 * kWaves, decode_waves_per_simd(G)) void split_kv_decode_map(
     MapArgs a, const uint32_t* __restrict__ page_ids, const uint32_t* __restrict__ kv_splits,
     const uint32_t* __restrict__ req_slots, const uint16_t* __restrict__ q, const uint16_t* __restrict__ pages,
@@ -262,6 +263,10 @@ __global__ __launch_bounds__(64 * kWaves, decode_waves_per_simd(G)) void split_k
 
     float* my_p = p_lds[wave];
     float* my_alpha = alpha_lds[wave];
+    float* logit_row = nullptr;
+    if constexpr (kLogits)
+        logit_row = a.logits + ((uint64_t)q_token * a.hq + (uint64_t)kv_head * G + (mt < (uint32_t)G ? mt : 0)) *
+                                   a.logits_stride;
 
     // One 16-token tile.  `partial`: the tile holds tokens outside [kv_begin, kv_end).
     // `has_next`: another tile of this wave follows; its K and V are requested on the way, each
@@ -291,6 +296,22 @@ __global__ __launch_bounds__(64 * kWaves, decode_waves_per_simd(G)) void split_k
             const bool valid = token >= lo && token < hi;
             v[r] = valid ? (s0[r] + s1[r]) * a.scale_log2 : -INFINITY;
             m = fmaxf(m, v[r]);
+        }
+        if constexpr (kLogits) {
+            // 64 contiguous bytes per query row and tile; the tile that a request's end or a row's border cuts is
+            // stored token by token
+            if (mt < (uint32_t)G) {
+                float* dst = logit_row + base + mc * 4;
+                if (!partial && base + kTileTokens <= a.logits_stride) {
+                    *reinterpret_cast<float4*>(dst) = make_float4(v[0], v[1], v[2], v[3]);
+                } else {
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        const uint32_t token = base + mc * 4 + r;
+                        if (token >= lo && token < hi && token < a.logits_stride) dst[r] = v[r];
+                    }
+                }
+            }
         }
         m = quarter_wave_max(m);
         const float next_max = fmaxf(run_max, m);
@@ -457,26 +478,26 @@ __global__ __launch_bounds__(64 * kWaves, decode_waves_per_simd(G)) void split_k
 }
 
 
-template <typename Tag, int D, int G>
+template <typename Tag, int D, int G, bool kLogits>
 inline void launch_decode_map_w(psi_hip_ctx* ctx, const Geometry& g, const MapArgs& a) {
     const dim3 grid((a.worker_cu ? a.num_workers : a.num_total_kv_splits) * g.hkv);
     const uint16_t* q = reinterpret_cast<const uint16_t*>(a.q);
     const uint16_t* pages = reinterpret_cast<const uint16_t*>(a.kv_pages);
     if (g.tokens_per_page == 8)  // a tile spans two pages
-        hipLaunchKernelGGL((split_kv_decode_map<Tag, D, G, 4, true>), grid, dim3(256), 0, ctx->stream, a,
+        hipLaunchKernelGGL((split_kv_decode_map<Tag, D, G, 4, true, kLogits>), grid, dim3(256), 0, ctx->stream, a,
                            a.walk.page_ids, a.kv_splits, a.req_slots, q, pages, a.worker_cu);
     else
-        hipLaunchKernelGGL((split_kv_decode_map<Tag, D, G, 4, false>), grid, dim3(256), 0, ctx->stream, a,
+        hipLaunchKernelGGL((split_kv_decode_map<Tag, D, G, 4, false, kLogits>), grid, dim3(256), 0, ctx->stream, a,
                            a.walk.page_ids, a.kv_splits, a.req_slots, q, pages, a.worker_cu);
 }
 
 // One translation unit per (element type, head_dim) instantiates every group size 1..8.
-template <typename Tag, int D>
+template <typename Tag, int D, bool kLogits = false>
 inline int launch_decode_map_group(psi_hip_ctx* ctx, const Geometry& g, const MapArgs& a) {
     switch (g.group) {
 #define PSI_CASE(G)                                        \
     case G:                                                \
-        launch_decode_map_w<Tag, D, G>(ctx, g, a);         \
+        launch_decode_map_w<Tag, D, G, kLogits>(ctx, g, a); \
         return PSI_HIP_OK;
         PSI_CASE(1)
         PSI_CASE(2)

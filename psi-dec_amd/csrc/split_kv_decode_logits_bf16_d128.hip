@@ -1,0 +1,8 @@
+// Instantiates the gfx950 decode map that stores its logits as well, for bf16 K/V, head_dim 128 (all group sizes).
+#include "split_kv_decode_kernel.h"
+
+namespace psi {
+int launch_decode_logits_bf16_d128(psi_hip_ctx* ctx, const Geometry& g, const MapArgs& a) {
+    return launch_decode_map_group<BF16Tag, 128, true>(ctx, g, a);
+}
+}  // namespace psi

@@ -62,28 +62,13 @@ __global__ __launch_bounds__(256) void store_partials_kernel(StorePartialsArgs a
     }
 }
 
-}  // namespace psi
-
-using namespace psi;
-
-extern "C" int psi_hip_split_kv_single_q_scratch_bytes(const psi_hip_gqa_config* cfg, uint32_t num_total_kv_splits,
-                                                       uint64_t* out_bytes) {
-    Geometry g;
-    int rc = make_geometry(cfg, &g);
-    if (rc != PSI_HIP_OK) return rc;
-    PSI_REQUIRE(out_bytes != nullptr, "out pointer must not be null");
-    PSI_REQUIRE(num_total_kv_splits > 0, "GQA SDPA requires KV splits");
-    *out_bytes = partial_layout(num_total_kv_splits, g.hq, g.d, 1).total_bytes;
-    return PSI_HIP_OK;
-}
-
-static int single_q_map_impl(psi_hip_ctx* ctx, const psi_hip_gqa_config* cfg, const psi_hip_page_table_layout* layout,
-                             const void* q, const void* kv_pages, uint64_t kv_pages_bytes, const uint32_t* req_slots,
-                             const uint32_t* page_ids, const uint32_t* kv_splits, const uint32_t* worker_cu,
-                             uint32_t num_workers, void* scratch, uint64_t scratch_bytes, uint32_t gqa_layer_index,
-                             uint32_t num_total_tokens, uint32_t num_total_kv_splits, uint32_t num_active_tokens,
-                             uint32_t num_active_kv_splits, const void* flat_k = nullptr, const void* flat_v = nullptr,
-                             const uint32_t* flat_token_indices = nullptr) {
+int single_q_map_impl(psi_hip_ctx* ctx, const psi_hip_gqa_config* cfg, const psi_hip_page_table_layout* layout,
+                      const void* q, const void* kv_pages, uint64_t kv_pages_bytes, const uint32_t* req_slots,
+                      const uint32_t* page_ids, const uint32_t* kv_splits, const uint32_t* worker_cu,
+                      uint32_t num_workers, void* scratch, uint64_t scratch_bytes, uint32_t gqa_layer_index,
+                      uint32_t num_total_tokens, uint32_t num_total_kv_splits, uint32_t num_active_tokens,
+                      uint32_t num_active_kv_splits, const void* flat_k, const void* flat_v,
+                      const uint32_t* flat_token_indices, float* logits, uint64_t logits_stride) {
     PSI_REQUIRE(ctx != nullptr, "ctx must not be null");
     Geometry g;
     int rc = make_geometry(cfg, &g);
@@ -125,6 +110,8 @@ static int single_q_map_impl(psi_hip_ctx* ctx, const psi_hip_gqa_config* cfg, co
     a.scale_log2 = g.scale * kLog2e;
     a.worker_cu = worker_cu;
     a.num_workers = num_workers;
+    a.logits = logits;
+    a.logits_stride = logits_stride;
     if (flat_k != nullptr) {
         // the append travels with the map when the MFMA kernel serves the shape, else it is a launch of its own
         a.flat_k = flat_k;
@@ -151,6 +138,21 @@ static int single_q_map_impl(psi_hip_ctx* ctx, const psi_hip_gqa_config* cfg, co
     }
     if (rc != PSI_HIP_OK) return rc;
     PSI_HIP_CHECK(hipGetLastError());
+    return PSI_HIP_OK;
+}
+
+}  // namespace psi
+
+using namespace psi;
+
+extern "C" int psi_hip_split_kv_single_q_scratch_bytes(const psi_hip_gqa_config* cfg, uint32_t num_total_kv_splits,
+                                                       uint64_t* out_bytes) {
+    Geometry g;
+    int rc = make_geometry(cfg, &g);
+    if (rc != PSI_HIP_OK) return rc;
+    PSI_REQUIRE(out_bytes != nullptr, "out pointer must not be null");
+    PSI_REQUIRE(num_total_kv_splits > 0, "GQA SDPA requires KV splits");
+    *out_bytes = partial_layout(num_total_kv_splits, g.hq, g.d, 1).total_bytes;
     return PSI_HIP_OK;
 }
 

@@ -1011,6 +1011,22 @@ class GQASplitKVSingleQScratch:
             self.buffer.fill_(fill)
 
 
+class GQASplitKVSingleQLogits:
+    """Room for the logits of the attention that accumulates weights (psi_hip_split_kv_single_q_logits_bytes):
+    `max_context_tokens` bounds the context of any token that it will serve."""
+
+    def __init__(self, device: Device, config: GQASplitKVSingleQConfig, shape: GQASplitKVSingleQShape,
+                 max_context_tokens: int):
+        import torch
+
+        out, cfg = ctypes.c_uint64(), config.struct()
+        L.check(device.lib.psi_hip_split_kv_single_q_logits_bytes(ctypes.byref(cfg), shape.num_total_tokens,
+                                                                  max_context_tokens, ctypes.byref(out)))
+        self.bytes, self.max_context_tokens = out.value, max_context_tokens
+        with torch.cuda.stream(device.stream):
+            self.buffer = torch.empty(self.bytes, dtype=torch.uint8, device=device.torch_device)
+
+
 class GQASplitKVSingleQKernels:
     def __init__(self, device: Device, config: GQASplitKVSingleQConfig, shape: GQASplitKVSingleQShape):
         config.num_tokens_per_page()
@@ -1077,6 +1093,26 @@ class GQASplitKVSingleQKernels:
             self.device.ctx, ctypes.byref(cfg), _ptr(scratch.buffer), scratch.bytes, _ptr(cu_sdpa_partial_outputs),
             _ptr(output), self.shape.num_total_tokens, self.shape.num_total_sdpa_map_task_templates,
             num_active_tokens, _ptr(partial_row_index), _gate_ref(gate)))
+
+    def invoke_attend_weights_bucketed(self, q, kv_pages, req_slots, flat_token_indices, page_ids,
+                                       sdpa_map_task_templates, cu_sdpa_partial_outputs, scratch,
+                                       logits: GQASplitKVSingleQLogits, output, page_weights, decay: float,
+                                       page_table_index: int, num_active_tokens: int, num_active_kv_splits: int,
+                                       worker_cu=None, num_workers: int = 0, flat_k=None, flat_v=None,
+                                       partial_row_index=None, gate: Optional["OutputGate"] = None):
+        """Map and combine (with the append folded in when `flat_k` / `flat_v` are given) that also add each cached
+        token's attention weight to `page_weights`, f32 [pages][KV heads][tokens per page] (see `eviction.py`):
+        tokens cached before this step keep `decay` times what they had, this step's own start from zero."""
+        cfg, layout = self.config.struct(), self.config.page_table_layout.struct()
+        weights = L.KVWeightsStruct(page_weights.data_ptr(), _nbytes(page_weights), logits.buffer.data_ptr(),
+                                    logits.bytes, logits.max_context_tokens, decay)
+        L.check(self.device.lib.psi_hip_split_kv_single_q_attend_weights(
+            self.device.ctx, ctypes.byref(cfg), ctypes.byref(layout), _ptr(q), _ptr(kv_pages), _nbytes(kv_pages),
+            _ptr(flat_k), _ptr(flat_v), _ptr(req_slots), _ptr(flat_token_indices), _ptr(page_ids),
+            _ptr(sdpa_map_task_templates), _ptr(cu_sdpa_partial_outputs), _ptr(worker_cu), num_workers,
+            _ptr(partial_row_index), _ptr(scratch.buffer), scratch.bytes, _ptr(output), _gate_ref(gate),
+            ctypes.byref(weights), page_table_index, self.shape.num_total_tokens,
+            self.shape.num_total_sdpa_map_task_templates, num_active_tokens, num_active_kv_splits))
 
 
 # ------------------------------------------------------------------ TiledQ verify / prefill
