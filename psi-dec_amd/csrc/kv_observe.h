@@ -1,0 +1,95 @@
+// Shared declarations of the observation kernels: attention weights of a window of query tokens over its request's
+// cached keys, summed per key and KV head and added to the accumulators, without the attention's output:
+//     w[h][p] = sum over the window's tokens t with p <= position(t), and over the query heads g of KV head h, of
+//               exp2(l[t][g][p] - lse[t][g]),   l = scale * log2(e) * q . k,   lse = log2 sum_p exp2(l).
+// The normaliser must be known before a weight is, so the keys are walked twice: a pass for the maximum and sum of every
+// (row, column), and a pass that joins those of a window's rows, recomputes the logits and sums the weights.  A row is a
+// range of keys of one window (psi_hip_kv_observe_plan), a column a (token of the window, query head of the KV head).  A
+// workgroup owns the accumulators of its row, so nothing is added atomically and the result does not depend on the order
+// of workgroups.
+#pragma once
+#include "kv_eviction.h"
+#include "split_kv.h"
+
+namespace psi {
+
+struct ObserveArgs {
+    CacheView v;
+    const void* q;
+    const void* pages;
+    const uint32_t* windows;
+    const uint32_t* rows;
+    uint32_t num_windows, num_rows, max_window, num_q_tokens;
+    uint32_t hq, group;
+    float scale_log2, decay;
+    float2* stats;  // [row][kv head][token in window][head of the group]: maximum (log2 domain) and sum
+    float* lse;     // [query row][q head], shape-generic kernels only
+    float* page_weights;
+    uint32_t* status;
+};
+
+// A maximum that no key contributes to: finite, so that no difference of two infinities arises.
+constexpr float kEmptyMax = -3.0e38f;
+
+// A window's row with every value that a wrong table could hold brought back into range.
+struct ObserveRow {
+    uint32_t slot, q_begin, num_q, position, held, begin, end, row_begin, row_end;
+    bool live;
+};
+__device__ __forceinline__ ObserveRow load_row(const ObserveArgs& a, uint32_t row) {
+    ObserveRow r;
+    const uint32_t w = a.rows[row * 3];
+    r.live = w < a.num_windows && a.windows[(uint64_t)w * kWindowWords] < a.v.num_slots;
+    const uint32_t* win = a.windows + (uint64_t)(r.live ? w : 0) * kWindowWords;
+    r.slot = win[0];
+    r.q_begin = min(win[1], a.num_q_tokens);
+    r.num_q = min(min(win[2], a.max_window), a.num_q_tokens - r.q_begin);
+    r.position = min(win[3], a.v.positions);
+    r.held = win[4];
+    r.row_begin = win[5];
+    r.row_end = min(win[6], a.num_rows);
+    r.begin = a.rows[row * 3 + 1];
+    r.end = min(min(a.rows[row * 3 + 2], r.position + r.num_q), a.v.positions);
+    return r;
+}
+
+__device__ __forceinline__ uint64_t stat_index(const ObserveArgs& a, uint32_t row, uint32_t kv_head, uint32_t column) {
+    return ((uint64_t)row * a.v.hkv + kv_head) * a.max_window * a.group + column;
+}
+
+// The normaliser of one column from its window's rows; +inf where no key contributes, so that its weights are zero.
+__device__ __forceinline__ float join_column(const ObserveArgs& a, const ObserveRow& r, uint32_t kv_head, uint32_t column) {
+    constexpr int kAhead = 8;
+    float m = kEmptyMax, s = 0.0f;
+    for (uint32_t row = r.row_begin; row < r.row_end; row += kAhead) {
+        float2 part[kAhead];
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u)
+            part[u] = row + u < r.row_end ? a.stats[stat_index(a, row + u, kv_head, column)] : make_float2(kEmptyMax, 0.0f);
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u) {
+            const float next = fmaxf(m, part[u].x);
+            s = s * exp2f(m - next) + part[u].y * exp2f(part[u].x - next);
+            m = next;
+        }
+    }
+    return s == 0.0f ? INFINITY : m + log2f(s);
+}
+
+// First weights of a position in this call: on top of what counts already.  Later ones: on top of the first.
+__device__ __forceinline__ void add_weight(const ObserveArgs& a, const ObserveRow& r, const uint32_t* table,
+                                           uint32_t kv_head, uint32_t p, float sum, bool first) {
+    const uint32_t page = page_of(a.v, table, p, a.v.num_weight_pages);
+    if (page == kNoPage) {
+        report_cache_range(a.status);
+        return;
+    }
+    float* acc = a.page_weights + weight_index(a.v, page, kv_head, page_place(a.v, p));
+    *acc = (!first ? *acc : p < r.held ? a.decay * *acc : 0.0f) + sum;
+}
+
+// Matrix-core kernels (kv_observe_kernel.h), one translation unit per element type; head_dim 128 or 256.
+void launch_observe_bf16(psi_hip_ctx* ctx, const ObserveArgs& a);
+void launch_observe_f16(psi_hip_ctx* ctx, const ObserveArgs& a);
+
+}  // namespace psi
