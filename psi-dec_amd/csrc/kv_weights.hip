@@ -5,7 +5,7 @@
 //               exp2(logit[t][g][p] - max[t][g]) / sum[t][g],
 // and adds them to the accumulators:  acc = (p appended before this step ? decay * acc : 0) + w.
 #include "kv_eviction.h"
-#include "split_kv.h"
+#include "split_kv_reduce_kernel.h"
 
 namespace psi {
 
@@ -27,71 +27,173 @@ struct WeightsArgs {
     uint32_t* status;
 };
 
+constexpr uint32_t kFinishThreads = 512, kFinishWaves = kFinishThreads / 64;
 constexpr uint32_t kLseEntries = 512;  // (token, head) normalisers held in LDS at a time
+constexpr uint32_t kFewEntries = 8;    // up to this many (a decode step's heads) a thread holds the logits of all
 
-// One workgroup per (kv_split row, KV head).  The rows of a request's last token of the step tile all its positions, so
-// those rows' workgroups own the accumulators they cover and the others have nothing to do: no two workgroups meet.
-__global__ __launch_bounds__(256) void accumulate_weights_kernel(WeightsArgs a) {
+// log2 of the sum of exponentials of one (token, head) over its partial states, in every lane of the wave; +inf where
+// nothing contributes, so that the row's weights are zero.
+__device__ __forceinline__ float lse_of(const WeightsArgs& a, uint32_t token, uint32_t head, uint32_t lane) {
+    const uint32_t p0 = a.cu_kv_splits[token], p1 = a.cu_kv_splits[token + 1];
+    float m = -INFINITY, s = 0.0f;
+    for (uint32_t p = p0 + lane; p < p1; p += 64) {
+        const uint64_t r = (uint64_t)(a.row_index ? a.row_index[p] : p) * a.hq + head;
+        const float pm = a.part_max[r], next = fmaxf(m, pm);
+        if (pm > -INFINITY) s = s * exp2f(m - next) + a.part_sum[r] * exp2f(pm - next);
+        m = next;
+    }
+#pragma unroll
+    for (int off = 32; off > 0; off >>= 1) {
+        const float om = __shfl_xor(m, off, 64), os = __shfl_xor(s, off, 64), next = fmaxf(m, om);
+        if (next > -INFINITY) s = s * exp2f(m - next) + os * exp2f(om - next);
+        m = next;
+    }
+    return m > -INFINITY ? m + log2f(s) : INFINITY;
+}
+
+// The accumulators of one (kv_split row, KV head), by a workgroup.  The rows of a request's last token of the step tile
+// all its positions, so those rows' workgroups own the accumulators they cover and the others have nothing to do: no two
+// workgroups meet.  A thread takes four adjacent positions at a time: logits, accumulators and stores of 16 bytes a lane
+// where a page holds a multiple of four tokens, and a whole row in one turn if it has up to 2048 keys.
+// The chain of dependent reads is what bounds it (table row -> tokens -> partial states -> logits -> accumulators, each a
+// round trip), so the first turn's logits and page IDs are asked for before the normalisers are.
+__device__ __forceinline__ void accumulate_row(const WeightsArgs& a, uint32_t split, uint32_t kv_head, float* lse) {
     const uint32_t num_tokens = active_count(a.replay_counts, kReplayTokens, a.num_active_tokens);
     const uint32_t num_splits = active_count(a.replay_counts, kReplaySplits, a.num_active_kv_splits);
     const uint32_t layer = active_layer(a.replay_counts, a.v.layer, a.v.num_layers);
-    const uint32_t split = blockIdx.x / a.v.hkv, kv_head = blockIdx.x % a.v.hkv;
     if (split >= num_splits) return;
-    const uint32_t token = a.kv_splits[split * 3];
+    const uint32_t token = a.kv_splits[split * 3], begin = a.kv_splits[split * 3 + 1], row_end = a.kv_splits[split * 3 + 2];
     if (token >= num_tokens) return;
     const uint32_t slot = a.req_slots[token];
     if (token + 1 < num_tokens && a.req_slots[token + 1] == slot) return;
     uint32_t first = token;
     while (first > 0 && a.req_slots[first - 1] == slot) --first;
-    const uint32_t held = a.flat_token_indices[first];
-    const uint32_t begin = a.kv_splits[split * 3 + 1];
-    const uint32_t row_end = a.kv_splits[split * 3 + 2], end = min(row_end, a.max_context);
+    const uint32_t held = a.flat_token_indices[first], own = a.flat_token_indices[token];
+    const uint32_t end = min(row_end, a.max_context);
     if (threadIdx.x == 0 && row_end > end) report_cache_range(a.status);
     const uint32_t* row = table_row(a.v, slot, layer);
-
-    __shared__ float lse[kLseEntries];
     const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const uint32_t entries = (token - first + 1) * a.group;
-    for (uint32_t base = 0; base < entries; base += kLseEntries) {
-        const uint32_t count = min(kLseEntries, entries - base);
-        for (uint32_t e = wave; e < count; e += 4) {
-            const uint32_t t = first + (base + e) / a.group, head = kv_head * a.group + (base + e) % a.group;
-            const uint32_t p0 = a.cu_kv_splits[t], p1 = a.cu_kv_splits[t + 1];
-            float m = -INFINITY, s = 0.0f;
-            for (uint32_t p = p0 + lane; p < p1; p += 64) {
-                const uint64_t r = (uint64_t)(a.row_index ? a.row_index[p] : p) * a.hq + head;
-                const float pm = a.part_max[r], next = fmaxf(m, pm);
-                if (pm > -INFINITY) s = s * exp2f(m - next) + a.part_sum[r] * exp2f(pm - next);
-                m = next;
-            }
-#pragma unroll
-            for (int off = 32; off > 0; off >>= 1) {
-                const float om = __shfl_xor(m, off, 64), os = __shfl_xor(s, off, 64), next = fmaxf(m, om);
-                if (next > -INFINITY) s = s * exp2f(m - next) + os * exp2f(om - next);
-                m = next;
-            }
-            // a row that nothing contributes to has weights of zero
-            if (lane == 0) lse[e] = m > -INFINITY ? m + log2f(s) : INFINITY;
-        }
-        __syncthreads();
-        for (uint32_t p = begin + threadIdx.x; p < end; p += 256) {
-            float sum = 0.0f;
-            for (uint32_t e = 0; e < count; ++e) {
-                const uint32_t t = first + (base + e) / a.group, head = kv_head * a.group + (base + e) % a.group;
-                if (p <= a.flat_token_indices[t])
-                    sum += exp2f(a.logits[((uint64_t)t * a.hq + head) * a.logits_stride + p] - lse[e]);
-            }
-            const uint32_t page = page_of(a.v, row, p, a.v.num_weight_pages);
+    const bool vector = a.v.log2_page < 32 && a.v.log2_page >= 2 && reinterpret_cast<uintptr_t>(a.page_weights) % 16 == 0;
+
+    // the accumulators of positions p .. p + 3, from `sum`; `first_turn`: on top of what counts already
+    auto add = [&](uint32_t p, const float (&sum)[4], uint32_t page, bool first_turn) {
+        if (vector && p >= begin && p + 4 <= end) {
             if (page == kNoPage) {
+                report_cache_range(a.status);
+                return;
+            }
+            float4* acc = reinterpret_cast<float4*>(a.page_weights + weight_index(a.v, page, kv_head, page_place(a.v, p)));
+            const float4 old = *acc;
+            auto base = [&](float x, uint32_t at) { return !first_turn ? x : at < held ? a.decay * x : 0.0f; };
+            *acc = make_float4(base(old.x, p) + sum[0], base(old.y, p + 1) + sum[1], base(old.z, p + 2) + sum[2],
+                               base(old.w, p + 3) + sum[3]);
+            return;
+        }
+#pragma unroll
+        for (uint32_t i = 0; i < 4; ++i) {
+            if (p + i < begin || p + i >= end) continue;
+            const uint32_t id = page_of(a.v, row, p + i, a.v.num_weight_pages);
+            if (id == kNoPage) {
                 report_cache_range(a.status);
                 continue;
             }
-            float* acc = a.page_weights + weight_index(a.v, page, kv_head, page_place(a.v, p));
-            const float old = base > 0 ? *acc : p < held ? a.decay * *acc : 0.0f;
-            *acc = old + sum;
+            float* acc = a.page_weights + weight_index(a.v, id, kv_head, page_place(a.v, p + i));
+            *acc = (!first_turn ? *acc : p + i < held ? a.decay * *acc : 0.0f) + sum[i];
+        }
+    };
+    const uint32_t start = (begin & ~3u) + threadIdx.x * 4;
+    const float* row_logits = a.logits + ((uint64_t)first * a.hq + kv_head * a.group) * a.logits_stride;
+
+    if (entries <= kFewEntries && token == first) {
+        // one token: its position is the row's last at most, so every key of the row is visible
+        float4 l[kFewEntries];
+        uint32_t page = kNoPage;
+        auto fetch = [&](uint32_t p) {
+#pragma unroll
+            for (uint32_t e = 0; e < kFewEntries; ++e)
+                if (e < entries) l[e] = *reinterpret_cast<const float4*>(row_logits + e * a.logits_stride + p);
+            page = page_of(a.v, row, p, a.v.num_weight_pages);
+        };
+        if (start < end) fetch(start);
+        if (wave < entries) {
+            const float x = lse_of(a, token, kv_head * a.group + wave, lane);
+            if (lane == 0) lse[wave] = x;
         }
         __syncthreads();
+        for (uint32_t p = start; p < end; p += kFinishThreads * 4) {
+            if (p != start) fetch(p);
+            float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (uint32_t e = 0; e < kFewEntries; ++e) {
+                if (e >= entries) continue;
+                const float x[4] = {l[e].x, l[e].y, l[e].z, l[e].w};
+#pragma unroll
+                for (int i = 0; i < 4; ++i) sum[i] += p + i <= own ? __builtin_amdgcn_exp2f(x[i] - lse[e]) : 0.0f;
+            }
+            add(p, sum, page, true);
+        }
+        return;
     }
+    for (uint32_t base = 0; base < entries; base += kLseEntries) {
+        const uint32_t count = min(kLseEntries, entries - base);
+        if (base > 0) __syncthreads();
+        for (uint32_t e = wave; e < count; e += kFinishWaves) {
+            const float x = lse_of(a, first + (base + e) / a.group, kv_head * a.group + (base + e) % a.group, lane);
+            if (lane == 0) lse[e] = x;
+        }
+        __syncthreads();
+        for (uint32_t p = start; p < end; p += kFinishThreads * 4) {
+            const uint32_t page = page_of(a.v, row, p, a.v.num_weight_pages);
+            float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+            uint32_t t = base / a.group, g = base % a.group;
+            for (uint32_t e = 0; e < count; ++e) {
+                const uint32_t last = a.flat_token_indices[first + t];
+                const float4 l = *reinterpret_cast<const float4*>(row_logits + ((uint64_t)t * a.hq + g) * a.logits_stride + p);
+                const float x[4] = {l.x, l.y, l.z, l.w};
+#pragma unroll
+                for (int i = 0; i < 4; ++i) sum[i] += p + i <= last ? __builtin_amdgcn_exp2f(x[i] - lse[e]) : 0.0f;
+                if (++g == a.group) {
+                    g = 0;
+                    ++t;
+                }
+            }
+            add(p, sum, page, base == 0);
+        }
+    }
+}
+
+// The combine and the accumulators in one launch: the first workgroups take a (kv_split row, KV head) each, the others
+// the output rows, a wave each or (kWide) a workgroup each, as the combine's own launch does.
+template <typename Tag, int D>
+__global__ __launch_bounds__(kFinishThreads) void finish_kernel(WeightsArgs w, ReduceArgs r, uint32_t weight_groups,
+                                                                uint32_t wide) {
+    __shared__ union {
+        float lse[kLseEntries];
+        WideReduceLds<D> wide;
+    } lds;
+    static_assert(kWideWaves == kFinishWaves, "a wide row takes the whole workgroup");
+    if (blockIdx.x < weight_groups) {
+        accumulate_row(w, blockIdx.x / w.v.hkv, blockIdx.x % w.v.hkv, lds.lse);
+        return;
+    }
+    resolve_active(r);
+    const uint64_t group = blockIdx.x - weight_groups;
+    if (wide) {
+        if (r.row_index != nullptr) reduce_row_wide<Tag, D, true>(r, group, lds.wide);
+        else reduce_row_wide<Tag, D, false>(r, group, lds.wide);
+        return;
+    }
+    const uint64_t row_out = group * kFinishWaves + (threadIdx.x >> 6);
+    if (row_out >= (uint64_t)r.num_active_tokens * r.hq) return;
+    if (r.row_index != nullptr) reduce_row<Tag, D, true>(r, row_out);
+    else reduce_row<Tag, D, false>(r, row_out);
+}
+
+// The accumulators alone, next to the shape-generic combine.
+__global__ __launch_bounds__(kFinishThreads) void accumulate_kernel(WeightsArgs w) {
+    __shared__ float lse[kLseEntries];
+    accumulate_row(w, blockIdx.x / w.v.hkv, blockIdx.x % w.v.hkv, lse);
 }
 
 static uint64_t logits_stride(uint32_t max_context_tokens) { return ((uint64_t)max_context_tokens + 15) / 16 * 16; }
@@ -136,6 +238,10 @@ extern "C" int psi_hip_split_kv_single_q_attend_weights(
     PSI_REQUIRE(weights->logits_bytes >= needed, "logits buffer too small: %llu < %llu",
                 (unsigned long long)weights->logits_bytes, (unsigned long long)needed);
     WeightsArgs a;
+    ReduceArgs r;
+    rc = single_q_reduce_args(ctx, cfg, scratch, scratch_bytes, cu_kv_splits, output, num_total_tokens,
+                              num_total_kv_splits, num_active_tokens, partial_row_index, gate, &g, &r);
+    if (rc != PSI_HIP_OK) return rc;
     rc = make_cache_view(g, layout, page_ids, gqa_layer_index, kv_pages_bytes, weights->page_weights_bytes, &a.v);
     if (rc != PSI_HIP_OK) return rc;
     PSI_REQUIRE((uint64_t)num_total_kv_splits * g.hkv <= 0x7fffffffull, "too many KV splits");
@@ -147,10 +253,6 @@ extern "C" int psi_hip_split_kv_single_q_attend_weights(
                            num_workers, scratch, scratch_bytes, gqa_layer_index, num_total_tokens, num_total_kv_splits,
                            num_active_tokens, num_active_kv_splits, flat_k, flat_v, flat_token_indices, logits, stride);
     if (rc != PSI_HIP_OK) return rc;
-    rc = psi_hip_split_kv_single_q_reduce(ctx, cfg, scratch, scratch_bytes, cu_kv_splits, output, num_total_tokens,
-                                          num_total_kv_splits, num_active_tokens, partial_row_index, gate);
-    if (rc != PSI_HIP_OK) return rc;
-
     const PartialLayout pl = partial_layout(num_total_kv_splits, g.hq, g.d, 1);
     a.logits = logits;
     a.logits_stride = stride;
@@ -170,8 +272,32 @@ extern "C" int psi_hip_split_kv_single_q_attend_weights(
     a.num_active_kv_splits = num_active_kv_splits;
     a.replay_counts = ctx->replay_counts;
     a.status = ctx->status_device;
+    const uint64_t weight_groups = (uint64_t)num_active_kv_splits * g.hkv;
+    const bool wide = reduce_is_wide(r);
+    const uint64_t rows = (uint64_t)num_active_tokens * g.hq, row_groups = wide ? rows : (rows + kFinishWaves - 1) / kFinishWaves;
+    if (ctx->force_generic || (g.d != 128 && g.d != 256) || weight_groups + row_groups > 0x7fffffffull) {
+        rc = launch_single_q_reduce(ctx, g, r);
+        if (rc != PSI_HIP_OK) return rc;
+        LaunchScope scope(ctx, "kv_weights");
+        hipLaunchKernelGGL(accumulate_kernel, dim3((uint32_t)weight_groups), dim3(kFinishThreads), 0, ctx->stream, a);
+        PSI_HIP_CHECK(hipGetLastError());
+        return PSI_HIP_OK;
+    }
     LaunchScope scope(ctx, "kv_weights");
-    hipLaunchKernelGGL(accumulate_weights_kernel, dim3(num_active_kv_splits * g.hkv), dim3(256), 0, ctx->stream, a);
+    const dim3 grid((uint32_t)(weight_groups + row_groups)), threads(kFinishThreads);
+#define PSI_FINISH(TAG)                                                                                                \
+    do {                                                                                                               \
+        if (g.d == 256)                                                                                                \
+            hipLaunchKernelGGL((finish_kernel<TAG, 256>), grid, threads, 0, ctx->stream, a, r, (uint32_t)weight_groups, \
+                               wide ? 1u : 0u);                                                                        \
+        else                                                                                                           \
+            hipLaunchKernelGGL((finish_kernel<TAG, 128>), grid, threads, 0, ctx->stream, a, r, (uint32_t)weight_groups, \
+                               wide ? 1u : 0u);                                                                        \
+    } while (0)
+    if (r.out_dtype == PSI_HIP_F32) PSI_FINISH(F32Tag);
+    else if (r.out_dtype == PSI_HIP_BF16) PSI_FINISH(BF16Tag);
+    else PSI_FINISH(F16Tag);
+#undef PSI_FINISH
     PSI_HIP_CHECK(hipGetLastError());
     return PSI_HIP_OK;
 }

@@ -112,6 +112,12 @@ struct ReduceArgs {
     const uint32_t* replay_counts = nullptr;  // see active_count()
 };
 
+// Long split lists on few tokens: a workgroup per output row of the combine instead of a wave.
+inline bool reduce_is_wide(const ReduceArgs& a) {
+    return a.num_active_tokens != 0 && a.num_total_kv_splits / a.num_active_tokens >= 32 &&
+           (uint64_t)a.num_active_tokens * a.hq <= 0x7fffffffull;
+}
+
 // First statement of every combine kernel.
 __device__ __forceinline__ void resolve_active(ReduceArgs& a) {
     a.num_active_tokens = active_count(a.replay_counts, kReplayTokens, a.num_active_tokens);
@@ -192,6 +198,13 @@ int single_q_map_impl(psi_hip_ctx* ctx, const psi_hip_gqa_config* cfg, const psi
                       uint32_t num_active_kv_splits, const void* flat_k = nullptr, const void* flat_v = nullptr,
                       const uint32_t* flat_token_indices = nullptr, float* logits = nullptr,
                       uint64_t logits_stride = 0);
+
+// The checks and kernel arguments of psi_hip_split_kv_single_q_reduce.
+int single_q_reduce_args(psi_hip_ctx* ctx, const psi_hip_gqa_config* cfg, const void* scratch, uint64_t scratch_bytes,
+                         const uint32_t* cu_kv_splits, void* output, uint32_t num_total_tokens,
+                         uint32_t num_total_kv_splits, uint32_t num_active_tokens, const uint32_t* partial_row_index,
+                         const psi_hip_output_gate* gate, Geometry* g, ReduceArgs* a);
+int launch_single_q_reduce(psi_hip_ctx* ctx, const Geometry& g, const ReduceArgs& a);
 
 // Fast decode map for head_dim 256 / 128, 2-byte elements, power-of-two pages; returns
 // PSI_HIP_ERR_UNSUPPORTED when the shape is outside its domain (caller falls back).

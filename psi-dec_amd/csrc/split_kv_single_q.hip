@@ -141,6 +141,49 @@ int single_q_map_impl(psi_hip_ctx* ctx, const psi_hip_gqa_config* cfg, const psi
     return PSI_HIP_OK;
 }
 
+int single_q_reduce_args(psi_hip_ctx* ctx, const psi_hip_gqa_config* cfg, const void* scratch, uint64_t scratch_bytes,
+                         const uint32_t* cu_kv_splits, void* output, uint32_t num_total_tokens,
+                         uint32_t num_total_kv_splits, uint32_t num_active_tokens, const uint32_t* partial_row_index,
+                         const psi_hip_output_gate* gate, Geometry* g, ReduceArgs* a) {
+    PSI_REQUIRE(ctx != nullptr, "ctx must not be null");
+    int rc = make_geometry(cfg, g);
+    if (rc != PSI_HIP_OK) return rc;
+    rc = check_single_q_shape(*g, num_total_tokens, num_total_kv_splits);
+    if (rc != PSI_HIP_OK) return rc;
+    PSI_REQUIRE(scratch && cu_kv_splits && output, "GQA SplitKV SingleQ reduce buffers must not be null");
+    PSI_REQUIRE(num_active_tokens > 0, "GQA SplitKV SingleQ active token count must be positive");
+    PSI_REQUIRE(num_active_tokens <= num_total_tokens,
+                "GQA SplitKV SingleQ active token count exceeds recorded capacity");
+    const PartialLayout pl = partial_layout(num_total_kv_splits, g->hq, g->d, 1);
+    PSI_REQUIRE(scratch_bytes >= pl.total_bytes, "GQA SplitKV SingleQ scratch too small: %llu < %llu",
+                (unsigned long long)scratch_bytes, (unsigned long long)pl.total_bytes);
+    a->part_max = reinterpret_cast<const float*>(static_cast<const char*>(scratch) + pl.max_offset);
+    a->part_sum = reinterpret_cast<const float*>(static_cast<const char*>(scratch) + pl.sum_offset);
+    a->part_acc = reinterpret_cast<const float*>(static_cast<const char*>(scratch) + pl.acc_offset);
+    a->cu_kv_splits = cu_kv_splits;
+    a->row_index = partial_row_index;
+    a->replay_counts = ctx->replay_counts;
+    a->output = output;
+    a->hq = g->hq;
+    a->d = g->d;
+    a->out_dtype = ctx->f32_output ? PSI_HIP_F32 : g->dtype;
+    a->num_active_tokens = num_active_tokens;
+    a->num_total_kv_splits = num_total_kv_splits;
+    return set_output_gate(a, gate, *g);
+}
+
+int launch_single_q_reduce(psi_hip_ctx* ctx, const Geometry& g, const ReduceArgs& a) {
+    LaunchScope scope(ctx, "split_kv_reduce");
+    int rc = launch_reduce_fast(ctx, g, a);
+    if (rc == PSI_HIP_ERR_UNSUPPORTED) {
+        launch_reduce_generic(ctx, g, a, 0);
+        rc = PSI_HIP_OK;
+    }
+    if (rc != PSI_HIP_OK) return rc;
+    PSI_HIP_CHECK(hipGetLastError());
+    return PSI_HIP_OK;
+}
+
 }  // namespace psi
 
 using namespace psi;
@@ -189,44 +232,12 @@ extern "C" int psi_hip_split_kv_single_q_reduce(psi_hip_ctx* ctx, const psi_hip_
                                                 uint32_t num_total_tokens, uint32_t num_total_kv_splits,
                                                 uint32_t num_active_tokens, const uint32_t* partial_row_index,
                                                 const psi_hip_output_gate* gate) {
-    PSI_REQUIRE(ctx != nullptr, "ctx must not be null");
     Geometry g;
-    int rc = make_geometry(cfg, &g);
-    if (rc != PSI_HIP_OK) return rc;
-    rc = check_single_q_shape(g, num_total_tokens, num_total_kv_splits);
-    if (rc != PSI_HIP_OK) return rc;
-    PSI_REQUIRE(scratch && cu_kv_splits && output, "GQA SplitKV SingleQ reduce buffers must not be null");
-    PSI_REQUIRE(num_active_tokens > 0, "GQA SplitKV SingleQ active token count must be positive");
-    PSI_REQUIRE(num_active_tokens <= num_total_tokens,
-                "GQA SplitKV SingleQ active token count exceeds recorded capacity");
-    const PartialLayout pl = partial_layout(num_total_kv_splits, g.hq, g.d, 1);
-    PSI_REQUIRE(scratch_bytes >= pl.total_bytes, "GQA SplitKV SingleQ scratch too small: %llu < %llu",
-                (unsigned long long)scratch_bytes, (unsigned long long)pl.total_bytes);
     ReduceArgs a;
-    a.part_max = reinterpret_cast<const float*>(static_cast<const char*>(scratch) + pl.max_offset);
-    a.part_sum = reinterpret_cast<const float*>(static_cast<const char*>(scratch) + pl.sum_offset);
-    a.part_acc = reinterpret_cast<const float*>(static_cast<const char*>(scratch) + pl.acc_offset);
-    a.cu_kv_splits = cu_kv_splits;
-    a.row_index = partial_row_index;
-    a.replay_counts = ctx->replay_counts;
-    a.output = output;
-    a.hq = g.hq;
-    a.d = g.d;
-    a.out_dtype = ctx->f32_output ? PSI_HIP_F32 : g.dtype;
-    a.num_active_tokens = num_active_tokens;
-    a.num_total_kv_splits = num_total_kv_splits;
-    rc = set_output_gate(&a, gate, g);
+    int rc = single_q_reduce_args(ctx, cfg, scratch, scratch_bytes, cu_kv_splits, output, num_total_tokens,
+                                  num_total_kv_splits, num_active_tokens, partial_row_index, gate, &g, &a);
     if (rc != PSI_HIP_OK) return rc;
-
-    LaunchScope scope(ctx, "split_kv_reduce");
-    rc = launch_reduce_fast(ctx, g, a);
-    if (rc == PSI_HIP_ERR_UNSUPPORTED) {
-        launch_reduce_generic(ctx, g, a, 0);
-        rc = PSI_HIP_OK;
-    }
-    if (rc != PSI_HIP_OK) return rc;
-    PSI_HIP_CHECK(hipGetLastError());
-    return PSI_HIP_OK;
+    return launch_single_q_reduce(ctx, g, a);
 }
 
 extern "C" int psi_hip_split_kv_single_q_store_partials(psi_hip_ctx* ctx, const psi_hip_gqa_config* cfg, void* scratch,
