@@ -881,14 +881,20 @@ int psi_hip_kv_evict_plan(const psi_hip_gqa_config* cfg, const psi_hip_page_tabl
                           const uint32_t* req_slots, const uint32_t* num_cached, uint32_t num_reqs, uint32_t* requests,
                           uint32_t* out_max_cached);
 
+/* Bytes of a selection's scratch (0 while no request holds more than 16384 tokens). */
+int psi_hip_kv_select_scratch_bytes(const psi_hip_gqa_config* cfg, uint32_t num_reqs, uint32_t max_cached_tokens,
+                                    uint64_t* out_bytes);
+
 /* kept: device u32[num_reqs][num_kv_heads][budget], the positions to keep in ascending order, padded with
  * PSI_HIP_SENTINEL: all of a request of up to `budget` tokens; of a longer one the first num_first, the last num_recent
  * (together at most budget) and the heaviest of the others, of equal weights the lower position.  NaN counts as -inf.
- * max_cached_tokens: the plan's.  Not while device-side counts are bound. */
+ * max_cached_tokens: the plan's.  scratch: device, 16-byte aligned, may be null when it needs no bytes.  Not while
+ * device-side counts are bound. */
 int psi_hip_kv_select_kept(psi_hip_ctx* ctx, const psi_hip_gqa_config* cfg, const psi_hip_page_table_layout* layout,
                            const float* page_weights, uint64_t page_weights_bytes, const uint32_t* page_ids,
                            const uint32_t* requests, uint32_t num_reqs, uint32_t max_cached_tokens, uint32_t budget,
-                           uint32_t num_first, uint32_t num_recent, uint32_t* kept, uint32_t gqa_layer_index);
+                           uint32_t num_first, uint32_t num_recent, uint32_t* kept, void* scratch,
+                           uint64_t scratch_bytes, uint32_t gqa_layer_index);
 
 /* Moves the K and V lines, and the accumulators unless page_weights is null, of position kept[i] to position i, in
  * place, for every request of more than `budget` tokens.  The kept positions of a (request, head) ascend, as the

@@ -2,8 +2,8 @@
 // the largest accumulated weight until `budget` are chosen; equal weights go to the lower position.  The chosen
 // positions come out in ascending order.  A NaN weight counts as -inf, -0 as 0.
 //
-// The budget-th largest weight is found by radix selection on order-preserving integer keys (eight bits a pass, the
-// histogram in LDS), the positions by ballots and prefix counts: no sort, and the same answer on every run.
+// The budget-th largest weight is found by radix selection on order-preserving integer keys (three digits, counted in
+// LDS), the positions by ballots and prefix counts: no sort, and the same answer on every run.
 #include "kv_eviction.h"
 
 namespace psi {
@@ -27,113 +27,322 @@ __device__ __forceinline__ uint32_t weight_key(float w) {
 constexpr uint32_t kKeepKey = 0xffffffffu;  // above every weight's key: tokens that are kept whatever their weight
 
 constexpr uint32_t kSelectThreads = 1024, kSelectWaves = kSelectThreads / 64;
+// Digits of a key, from the top: 11, 11 and 10 bits.  The first one holds the sign, the exponent and two bits of the
+// mantissa, so that accumulated weights, which span few exponents, still spread over some tens of counters.
+constexpr uint32_t kBins = 2048;
+constexpr int kDigits = 3;
+__device__ __forceinline__ uint32_t digit_shift(int d) { return d == 0 ? 21 : d == 1 ? 10 : 0; }
+__device__ __forceinline__ uint32_t digit_of(uint32_t key, int d) { return d == 2 ? key & 1023 : key >> digit_shift(d) & 2047; }
 
-// One workgroup per (request, KV head).
-__global__ __launch_bounds__(kSelectThreads) void select_kept_kernel(SelectArgs a) {
-    const uint32_t req = blockIdx.x / a.v.hkv, kv_head = blockIdx.x % a.v.hkv;
-    const uint32_t slot = a.requests[req * kRequestWords], n = min(min(a.requests[req * kRequestWords + 1], a.max_cached), a.v.positions);
-    uint32_t* kept = a.kept + (uint64_t)blockIdx.x * a.budget;
-    const uint32_t tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    for (uint32_t i = min(n, a.budget) + tid; i < a.budget; i += kSelectThreads) kept[i] = PSI_HIP_SENTINEL;
-    if (slot >= a.v.num_slots) {
-        for (uint32_t i = tid; i < min(n, a.budget); i += kSelectThreads) kept[i] = PSI_HIP_SENTINEL;
-        report_cache_range(a.status);
-        return;
+struct SelectRow {
+    const uint32_t* table;
+    uint32_t kv_head, n, recent_from;
+    bool vector;  // four adjacent positions share a page and a 16-byte aligned address
+};
+__device__ __forceinline__ SelectRow make_row(const SelectArgs& a, uint32_t slot, uint32_t kv_head, uint32_t n) {
+    SelectRow r;
+    r.table = table_row(a.v, slot, a.v.layer);
+    r.kv_head = kv_head;
+    r.n = n;
+    r.recent_from = n - min(a.num_recent, n);
+    r.vector = a.v.log2_page < 32 && a.v.log2_page >= 2 && reinterpret_cast<uintptr_t>(a.page_weights) % 16 == 0;
+    return r;
+}
+
+// Keys of positions p .. p + 3 (p a multiple of four); of positions from n on: 0, which no weight has (-inf's is higher).
+__device__ __forceinline__ void load_keys(const SelectArgs& a, const SelectRow& r, uint32_t p, uint32_t (&key)[4]) {
+    float w[4];
+    uint32_t missing = 0;
+    if (r.vector) {
+        const uint32_t page = p < r.n ? page_of(a.v, r.table, p, a.v.num_weight_pages) : kNoPage;
+        float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        if (page != kNoPage)
+            x = *reinterpret_cast<const float4*>(a.page_weights + weight_index(a.v, page, r.kv_head, page_place(a.v, p)));
+        else missing = 15;
+        w[0] = x.x;
+        w[1] = x.y;
+        w[2] = x.z;
+        w[3] = x.w;
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const uint32_t page = p + i < r.n ? page_of(a.v, r.table, p + i, a.v.num_weight_pages) : kNoPage;
+            w[i] = 0.0f;
+            if (page != kNoPage) w[i] = a.page_weights[weight_index(a.v, page, r.kv_head, page_place(a.v, p + i))];
+            else missing |= 1u << i;
+        }
     }
-    if (n <= a.budget) {
-        for (uint32_t i = tid; i < n; i += kSelectThreads) kept[i] = i;
-        return;
-    }
-    const uint32_t* row = table_row(a.v, slot, a.v.layer);
-    const uint32_t recent_from = n - min(a.num_recent, n);
-    auto key_of = [&](uint32_t p) -> uint32_t {
-        if (p < a.num_first || p >= recent_from) return kKeepKey;
-        const uint32_t page = page_of(a.v, row, p, a.v.num_weight_pages);
-        if (page == kNoPage) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const bool always = p + i < a.num_first || p + i >= r.recent_from;
+        if ((missing >> i & 1) && !always && p + i < r.n) {  // counts as the lightest
+            w[i] = -INFINITY;
             report_cache_range(a.status);
-            return weight_key(-INFINITY);
         }
-        return weight_key(a.page_weights[weight_index(a.v, page, kv_head, page_place(a.v, p))]);
-    };
-
-    __shared__ uint32_t hist[256];
-    __shared__ uint32_t above[256];
-    __shared__ uint32_t chosen[2];
-    __shared__ uint32_t wave_gt[kSelectWaves], wave_eq[kSelectWaves];
-    uint32_t prefix = 0, remaining = a.budget;
-    for (int shift = 24; shift >= 0; shift -= 8) {
-        if (tid < 256) hist[tid] = 0;
-        __syncthreads();
-        for (uint32_t p = tid; p < n; p += kSelectThreads) {
-            const uint32_t key = key_of(p);
-            if (shift == 24 || (key >> (shift + 8)) == prefix) atomicAdd(&hist[(key >> shift) & 255], 1u);
-        }
-        __syncthreads();
-        if (tid < 256) above[tid] = hist[tid];
-        __syncthreads();
-        // above[b] = keys in bins b and higher
-        for (uint32_t step = 1; step < 256; step <<= 1) {
-            uint32_t add = 0;
-            if (tid < 256 && tid + step < 256) add = above[tid + step];
-            __syncthreads();
-            if (tid < 256) above[tid] += add;
-            __syncthreads();
-        }
-        if (tid < 256) {
-            const uint32_t higher = tid < 255 ? above[tid + 1] : 0;
-            if (above[tid] >= remaining && higher < remaining) {
-                chosen[0] = tid;
-                chosen[1] = remaining - higher;
-            }
-        }
-        __syncthreads();
-        prefix = prefix << 8 | chosen[0];
-        remaining = chosen[1];
-        __syncthreads();
-    }
-    // `remaining` of the keys equal to the threshold belong to the kept ones: those at the lowest positions
-    const uint32_t threshold = prefix;
-    const uint32_t share = (n + kSelectThreads - 1) / kSelectThreads * 64;
-    const uint32_t begin = min(wave * share, n), end = min(begin + share, n);
-    uint32_t gt = 0, eq = 0;
-    for (uint32_t base = begin; base < end; base += 64) {
-        const uint32_t p = base + lane;
-        const uint32_t key = p < end ? key_of(p) : 0;
-        gt += __popcll(__ballot(p < end && key > threshold));
-        eq += __popcll(__ballot(p < end && key == threshold));
-    }
-    if (lane == 0) {
-        wave_gt[wave] = gt;
-        wave_eq[wave] = eq;
-    }
-    __syncthreads();
-    uint32_t gt_before = 0, eq_before = 0;
-    for (uint32_t w = 0; w < wave; ++w) {
-        gt_before += wave_gt[w];
-        eq_before += wave_eq[w];
-    }
-    const uint64_t lower = ((uint64_t)1 << lane) - 1;
-    for (uint32_t base = begin; base < end; base += 64) {
-        const uint32_t p = base + lane;
-        const uint32_t key = p < end ? key_of(p) : 0;
-        const uint64_t gt_mask = __ballot(p < end && key > threshold), eq_mask = __ballot(p < end && key == threshold);
-        const uint32_t eq_rank = eq_before + __popcll(eq_mask & lower);
-        const uint32_t at = gt_before + __popcll(gt_mask & lower) + min(eq_rank, remaining);
-        if (p < end && (key > threshold || (key == threshold && eq_rank < remaining)) && at < a.budget) kept[at] = p;
-        gt_before += __popcll(gt_mask);
-        eq_before += __popcll(eq_mask);
+        key[i] = p + i >= r.n ? 0u : always ? kKeepKey : weight_key(w[i]);
     }
 }
+
+// What the selection of one row has settled after some digits: the keys to keep are those whose leading bits exceed
+// `prefix`, and `remaining` of those whose leading bits equal it.
+struct SelectState {
+    uint32_t prefix, remaining;
+};
+__device__ __forceinline__ bool matches(uint32_t key, int digit, uint32_t prefix) {
+    return digit == 0 || key >> digit_shift(digit - 1) == prefix;
+}
+
+struct BinSearch {
+    uint32_t totals[kSelectWaves];
+    uint32_t chosen[2];
+};
+// The counter that the `remaining`-th largest key falls into, and how many of that counter's keys are still to be kept.
+// Thread t brings the counts of the two highest counters it has not been beaten to: counters kBins - 1 - 2t and the one
+// below.  Returns the exclusive sum over the counters above the thread's in `above`.
+__device__ __forceinline__ void find_bin(BinSearch& lds, uint32_t tid, uint32_t high, uint32_t low, SelectState& st, int digit) {
+    const uint32_t lane = tid & 63, wave = tid >> 6;
+    uint32_t sum = high + low;
+#pragma unroll
+    for (int off = 1; off < 64; off <<= 1) {
+        const uint32_t other = __shfl_up(sum, off, 64);
+        if ((int)lane >= off) sum += other;
+    }
+    if (lane == 63) lds.totals[wave] = sum;
+    __syncthreads();
+    uint32_t above = sum - high - low;
+    for (uint32_t w = 0; w < wave; ++w) above += lds.totals[w];
+    if (above < st.remaining && st.remaining <= above + high + low) {
+        const bool first = st.remaining <= above + high;
+        lds.chosen[0] = kBins - 1 - 2 * tid - (first ? 0 : 1);
+        lds.chosen[1] = st.remaining - above - (first ? 0 : high);
+    }
+    __syncthreads();
+    st.prefix = digit == 2 ? st.prefix << 10 | lds.chosen[0] : st.prefix << 11 | lds.chosen[0];
+    st.remaining = lds.chosen[1];
+}
+
+// What every selection starts with: the row's request, the padding behind what it keeps, and the rows that keep all.
+// False: nothing is left to do.
+__device__ __forceinline__ bool begin_row(const SelectArgs& a, uint32_t row, bool writes, SelectRow* r, uint32_t** kept) {
+    const uint32_t req = row / a.v.hkv, slot = a.requests[req * kRequestWords];
+    const uint32_t n = min(min(a.requests[req * kRequestWords + 1], a.max_cached), a.v.positions);
+    *kept = a.kept + (uint64_t)row * a.budget;
+    const bool valid = slot < a.v.num_slots;
+    if (writes) {
+        const uint32_t filled = valid ? min(n, a.budget) : 0;
+        for (uint32_t i = filled + threadIdx.x; i < a.budget; i += kSelectThreads) (*kept)[i] = PSI_HIP_SENTINEL;
+        if (valid && n <= a.budget)
+            for (uint32_t i = threadIdx.x; i < n; i += kSelectThreads) (*kept)[i] = i;
+        if (!valid) report_cache_range(a.status);
+    }
+    if (!valid || n <= a.budget) return false;
+    *r = make_row(a, slot, row % a.v.hkv, n);
+    return true;
+}
+
+// Writes the kept positions among the four keys a thread holds in each of kQuads turns (turn q, thread t: positions
+// first + 4 (q * 1024 + t) ..).  gt_before, eq_before: keys above and equal to the threshold ahead of `first`; of the equal
+// ones the first `take` are kept.
+struct EmitLds {
+    uint32_t gt[16 * kSelectWaves], eq[16 * kSelectWaves];
+};
+template <int kQuads>
+__device__ __forceinline__ void emit(const SelectArgs& a, EmitLds& lds, const uint32_t (&key)[kQuads][4], uint32_t first,
+                                     uint32_t threshold, uint32_t take, uint32_t gt_before, uint32_t eq_before,
+                                     uint32_t* kept) {
+    static_assert(kQuads <= 16, "turns of a thread");
+    const uint32_t tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const uint64_t lower = ((uint64_t)1 << lane) - 1;
+    auto lanes_below = [&](uint32_t count, uint32_t* total) {  // sum over the lower lanes and over the wave; count <= 4
+        const uint64_t b0 = __ballot(count & 1), b1 = __ballot(count & 2), b2 = __ballot(count & 4);
+        *total = __popcll(b0) + 2 * __popcll(b1) + 4 * __popcll(b2);
+        return (uint32_t)(__popcll(b0 & lower) + 2 * __popcll(b1 & lower) + 4 * __popcll(b2 & lower));
+    };
+    uint32_t gt_at[kQuads], eq_at[kQuads];
+#pragma unroll
+    for (int q = 0; q < kQuads; ++q) {
+        uint32_t gt = 0, eq = 0, total;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            gt += key[q][i] > threshold;
+            eq += key[q][i] == threshold;
+        }
+        gt_at[q] = lanes_below(gt, &total);
+        if (lane == 0) lds.gt[q * kSelectWaves + wave] = total;
+        eq_at[q] = lanes_below(eq, &total);
+        if (lane == 0) lds.eq[q * kSelectWaves + wave] = total;
+    }
+    __syncthreads();
+    for (uint32_t w = 0; w < wave; ++w) {
+        gt_before += lds.gt[w];
+        eq_before += lds.eq[w];
+    }
+#pragma unroll
+    for (int q = 0; q < kQuads; ++q) {
+        uint32_t gt = gt_before + gt_at[q], eq = eq_before + eq_at[q];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const bool above = key[q][i] > threshold, equal = key[q][i] == threshold;
+            const uint32_t at = gt + min(eq, take);
+            if ((above || (equal && eq < take)) && at < a.budget) kept[at] = first + 4 * (q * kSelectThreads + tid) + i;
+            gt += above;
+            eq += equal;
+        }
+        if (q + 1 < kQuads)
+            for (uint32_t w = wave; w < wave + kSelectWaves; ++w) {  // the waves from this one on, then the next turn's first
+                gt_before += lds.gt[q * kSelectWaves + w];
+                eq_before += lds.eq[q * kSelectWaves + w];
+            }
+    }
+}
+
+// Counters in LDS, four copies that the lanes share out, so that the lanes of a wave that meet in a counter are fewer.
+constexpr uint32_t kCopies = 4;
+__device__ __forceinline__ void clear_bins(uint32_t* hist, uint32_t tid) {
+    uint4* h = reinterpret_cast<uint4*>(hist);
+    for (uint32_t i = tid; i < kCopies * kBins / 4; i += kSelectThreads) h[i] = make_uint4(0, 0, 0, 0);
+}
+__device__ __forceinline__ uint32_t bin_count(const uint32_t* hist, uint32_t bin) {
+    uint32_t sum = 0;
+#pragma unroll
+    for (uint32_t c = 0; c < kCopies; ++c) sum += hist[c * kBins + bin];
+    return sum;
+}
+template <int kQuads>
+__device__ __forceinline__ void count_digits(uint32_t* hist, const uint32_t (&key)[kQuads][4], int digit, uint32_t prefix) {
+    uint32_t* mine = hist + (threadIdx.x % kCopies) * kBins;
+#pragma unroll
+    for (int q = 0; q < kQuads; ++q)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (key[q][i] != 0 && matches(key[q][i], digit, prefix)) atomicAdd(&mine[digit_of(key[q][i], digit)], 1u);
+}
+
+// One workgroup per (request, KV head), its keys in registers: rows of up to 4096 * kQuads positions.
+template <int kQuads>
+__global__ __launch_bounds__(kSelectThreads) void select_row_kernel(SelectArgs a) {
+    __shared__ __attribute__((aligned(16))) uint32_t hist[kCopies * kBins];
+    __shared__ BinSearch search;
+    __shared__ EmitLds emit_lds;
+    SelectRow r;
+    uint32_t* kept;
+    if (!begin_row(a, blockIdx.x, true, &r, &kept)) return;
+    const uint32_t tid = threadIdx.x;
+    uint32_t key[kQuads][4];
+#pragma unroll
+    for (int q = 0; q < kQuads; ++q) load_keys(a, r, 4 * (q * kSelectThreads + tid), key[q]);
+    SelectState st = {0, a.budget};
+    for (int digit = 0; digit < kDigits; ++digit) {
+        clear_bins(hist, tid);
+        __syncthreads();
+        count_digits<kQuads>(hist, key, digit, st.prefix);
+        __syncthreads();
+        find_bin(search, tid, bin_count(hist, kBins - 1 - 2 * tid), bin_count(hist, kBins - 2 - 2 * tid), st, digit);
+    }
+    emit<kQuads>(a, emit_lds, key, 0, st.prefix, st.remaining, 0, 0, kept);
+}
+
+// Longer rows: a workgroup per (row, chunk of 8192 positions) and a launch per digit.  Each launch adds up the counters
+// that the one before left for every chunk of the row, which gives the digit's value and, from the chunks ahead, the
+// number of kept positions before this chunk's first; so nothing is cleared or added atomically in memory.
+constexpr int kChunkQuads = 2;
+constexpr uint32_t kChunkKeys = 4 * kChunkQuads * kSelectThreads;
+struct ChunkState {
+    uint32_t prefix, remaining, gt_before, unused;
+};
+__host__ __device__ inline uint64_t select_chunks(uint32_t max_cached) { return ((uint64_t)max_cached + kChunkKeys - 1) / kChunkKeys; }
+
+// kPass 0 .. 2: counts digit kPass; kPass 3: writes the positions.
+template <int kPass>
+__global__ __launch_bounds__(kSelectThreads) void select_chunk_kernel(SelectArgs a, uint32_t num_chunks, uint32_t* hists,
+                                                                      ChunkState* states) {
+    __shared__ __attribute__((aligned(16))) uint32_t hist[kCopies * kBins];
+    __shared__ BinSearch search;
+    __shared__ EmitLds emit_lds;
+    __shared__ uint32_t wave_sum[kSelectWaves], equal_before;
+    const uint32_t row = blockIdx.x / num_chunks, chunk = blockIdx.x % num_chunks, tid = threadIdx.x;
+    SelectRow r;
+    uint32_t* kept;
+    if (!begin_row(a, row, kPass == 0 && chunk == 0, &r, &kept)) return;
+    const uint32_t first = chunk * kChunkKeys, row_chunks = (r.n + kChunkKeys - 1) / kChunkKeys;
+    if (chunk >= row_chunks) return;
+    const uint64_t rows = gridDim.x / num_chunks;
+    auto bins_of = [&](int digit, uint32_t c) { return hists + ((digit * rows + row) * num_chunks + c) * kBins; };
+    uint32_t key[kChunkQuads][4];
+#pragma unroll
+    for (int q = 0; q < kChunkQuads; ++q) load_keys(a, r, first + 4 * (q * kSelectThreads + tid), key[q]);
+
+    SelectState st = {0, a.budget};
+    uint32_t gt_before = 0;
+    if constexpr (kPass > 0) {
+        ChunkState* mine = states + row * (uint64_t)num_chunks + chunk;
+        if (kPass > 1) {
+            const ChunkState s = *mine;
+            st = {s.prefix, s.remaining};
+            gt_before = s.gt_before;
+        }
+        // counters kBins - 1 - 2t and the one below: over the row, and over the chunks ahead
+        uint32_t high = 0, low = 0, high_ahead = 0, low_ahead = 0;
+        const uint32_t at = kBins - 2 - 2 * tid;
+        for (uint32_t c = 0; c < row_chunks; ++c) {
+            const uint2 v = *reinterpret_cast<const uint2*>(bins_of(kPass - 1, c) + at);
+            low += v.x;
+            high += v.y;
+            if (c < chunk) {
+                low_ahead += v.x;
+                high_ahead += v.y;
+            }
+        }
+        find_bin(search, tid, high, low, st, kPass - 1);
+        // keys ahead whose digit exceeds the chosen one, and (last digit) those that equal the threshold
+        const uint32_t bin = search.chosen[0];
+        uint32_t ahead = (at + 1 > bin ? high_ahead : 0) + (at > bin ? low_ahead : 0);
+        if (at == bin) equal_before = low_ahead;
+        if (at + 1 == bin) equal_before = high_ahead;
+#pragma unroll
+        for (int off = 32; off > 0; off >>= 1) ahead += __shfl_xor(ahead, off, 64);
+        if ((tid & 63) == 0) wave_sum[tid >> 6] = ahead;
+        __syncthreads();
+        for (uint32_t w = 0; w < kSelectWaves; ++w) gt_before += wave_sum[w];
+        if (kPass < 3 && tid == 0) *mine = {st.prefix, st.remaining, gt_before, 0};
+    }
+    if constexpr (kPass < 3) {
+        clear_bins(hist, tid);
+        __syncthreads();
+        count_digits<kChunkQuads>(hist, key, kPass, st.prefix);
+        __syncthreads();
+        uint32_t* out = bins_of(kPass, chunk);
+        for (uint32_t b = tid; b < kBins; b += kSelectThreads) out[b] = bin_count(hist, b);
+    } else {
+        emit<kChunkQuads>(a, emit_lds, key, first, st.prefix, st.remaining, gt_before, equal_before, kept);
+    }
+}
+
+// Rows of up to this many positions go to one workgroup each.
+constexpr uint32_t kRowPositions = 16384;
 
 }  // namespace psi
 
 using namespace psi;
 
+extern "C" int psi_hip_kv_select_scratch_bytes(const psi_hip_gqa_config* cfg, uint32_t num_reqs,
+                                               uint32_t max_cached_tokens, uint64_t* out_bytes) {
+    Geometry g;
+    int rc = make_geometry(cfg, &g);
+    if (rc != PSI_HIP_OK) return rc;
+    PSI_REQUIRE(out_bytes != nullptr, "out pointer must not be null");
+    PSI_REQUIRE(num_reqs > 0, "a selection needs requests");
+    const uint64_t chunks = (uint64_t)num_reqs * g.hkv * select_chunks(max_cached_tokens);
+    *out_bytes = max_cached_tokens <= kRowPositions ? 0 : chunks * (kDigits * kBins * 4 + sizeof(ChunkState));
+    return PSI_HIP_OK;
+}
+
 extern "C" int psi_hip_kv_select_kept(psi_hip_ctx* ctx, const psi_hip_gqa_config* cfg,
                                       const psi_hip_page_table_layout* layout, const float* page_weights,
                                       uint64_t page_weights_bytes, const uint32_t* page_ids, const uint32_t* requests,
                                       uint32_t num_reqs, uint32_t max_cached_tokens, uint32_t budget, uint32_t num_first,
-                                      uint32_t num_recent, uint32_t* kept, uint32_t gqa_layer_index) {
+                                      uint32_t num_recent, uint32_t* kept, void* scratch, uint64_t scratch_bytes,
+                                      uint32_t gqa_layer_index) {
     PSI_REQUIRE(ctx != nullptr, "ctx must not be null");
     Geometry g;
     int rc = make_geometry(cfg, &g);
@@ -157,9 +366,33 @@ extern "C" int psi_hip_kv_select_kept(psi_hip_ctx* ctx, const psi_hip_gqa_config
     a.budget = budget;
     a.num_first = num_first;
     a.num_recent = num_recent;
+    uint64_t needed = 0;
+    rc = psi_hip_kv_select_scratch_bytes(cfg, num_reqs, max_cached_tokens, &needed);
+    if (rc != PSI_HIP_OK) return rc;
+    PSI_REQUIRE(scratch_bytes >= needed && (needed == 0 || scratch != nullptr), "selection scratch too small: %llu < %llu",
+                (unsigned long long)scratch_bytes, (unsigned long long)needed);
+    PSI_REQUIRE(reinterpret_cast<uintptr_t>(scratch) % 16 == 0, "the selection scratch must be 16-byte aligned");
+    const uint32_t rows = num_reqs * g.hkv;
     DeviceGuard guard(ctx->device);
     LaunchScope scope(ctx, "kv_select");
-    hipLaunchKernelGGL(select_kept_kernel, dim3(num_reqs * g.hkv), dim3(kSelectThreads), 0, ctx->stream, a);
+    const dim3 threads(kSelectThreads);
+    if (max_cached_tokens <= 4096) {
+        hipLaunchKernelGGL(select_row_kernel<1>, dim3(rows), threads, 0, ctx->stream, a);
+    } else if (max_cached_tokens <= 8192) {
+        hipLaunchKernelGGL(select_row_kernel<2>, dim3(rows), threads, 0, ctx->stream, a);
+    } else if (max_cached_tokens <= kRowPositions) {
+        hipLaunchKernelGGL(select_row_kernel<4>, dim3(rows), threads, 0, ctx->stream, a);
+    } else {
+        const uint64_t chunks = select_chunks(max_cached_tokens), grid = rows * chunks;
+        PSI_REQUIRE(grid <= 0x7fffffffull, "too many requests of this length in one selection");
+        uint32_t* hists = static_cast<uint32_t*>(scratch);
+        ChunkState* states = reinterpret_cast<ChunkState*>(hists + grid * kDigits * kBins);
+        const dim3 blocks((uint32_t)grid);
+        hipLaunchKernelGGL(select_chunk_kernel<0>, blocks, threads, 0, ctx->stream, a, (uint32_t)chunks, hists, states);
+        hipLaunchKernelGGL(select_chunk_kernel<1>, blocks, threads, 0, ctx->stream, a, (uint32_t)chunks, hists, states);
+        hipLaunchKernelGGL(select_chunk_kernel<2>, blocks, threads, 0, ctx->stream, a, (uint32_t)chunks, hists, states);
+        hipLaunchKernelGGL(select_chunk_kernel<3>, blocks, threads, 0, ctx->stream, a, (uint32_t)chunks, hists, states);
+    }
     PSI_HIP_CHECK(hipGetLastError());
     return PSI_HIP_OK;
 }

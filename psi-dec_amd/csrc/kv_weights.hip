@@ -103,16 +103,16 @@ __device__ __forceinline__ void accumulate_row(const WeightsArgs& a, uint32_t sp
         }
     };
     const uint32_t start = (begin & ~3u) + threadIdx.x * 4;
-    const float* row_logits = a.logits + ((uint64_t)first * a.hq + kv_head * a.group) * a.logits_stride;
 
     if (entries <= kFewEntries && token == first) {
         // one token: its position is the row's last at most, so every key of the row is visible
+        const float* token_logits = a.logits + logit_index(a.logits_stride, a.group, (uint64_t)token * a.v.hkv + kv_head, 0, 0);
         float4 l[kFewEntries];
         uint32_t page = kNoPage;
         auto fetch = [&](uint32_t p) {
 #pragma unroll
             for (uint32_t e = 0; e < kFewEntries; ++e)
-                if (e < entries) l[e] = *reinterpret_cast<const float4*>(row_logits + e * a.logits_stride + p);
+                if (e < entries) l[e] = *reinterpret_cast<const float4*>(token_logits + (uint64_t)p * a.group + e * 4);
             page = page_of(a.v, row, p, a.v.num_weight_pages);
         };
         if (start < end) fetch(start);
@@ -149,7 +149,8 @@ __device__ __forceinline__ void accumulate_row(const WeightsArgs& a, uint32_t sp
             uint32_t t = base / a.group, g = base % a.group;
             for (uint32_t e = 0; e < count; ++e) {
                 const uint32_t last = a.flat_token_indices[first + t];
-                const float4 l = *reinterpret_cast<const float4*>(row_logits + ((uint64_t)t * a.hq + g) * a.logits_stride + p);
+                const float4 l = *reinterpret_cast<const float4*>(
+                    a.logits + logit_index(a.logits_stride, a.group, (uint64_t)(first + t) * a.v.hkv + kv_head, p, g));
                 const float x[4] = {l.x, l.y, l.z, l.w};
 #pragma unroll
                 for (int i = 0; i < 4; ++i) sum[i] += p + i <= last ? __builtin_amdgcn_exp2f(x[i] - lse[e]) : 0.0f;

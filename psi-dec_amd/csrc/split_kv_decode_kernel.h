@@ -97,7 +97,10 @@ __device__ __forceinline__ void wave_lds_fence() { asm volatile("s_waitcnt lgkmc
 // KV head; six to eight need 172 to 198 registers and would spill, and a kernel with a private segment starts far
 // slower than one resident wave less costs (two and three workgroups per SIMD stream equally fast), so those
 // are held to two.
-constexpr int decode_waves_per_simd(int group) { return group > 5 ? 2 : PSI_DECODE_WAVES_PER_SIMD; }
+// Storing the logits takes a few registers more, which four and five heads have not left either.
+constexpr int decode_waves_per_simd(int group, bool logits = false) {
+    return group > (logits ? 3 : 5) ? 2 : PSI_DECODE_WAVES_PER_SIMD;
+}
 
 constexpr int kTileTokens = 16;
 
@@ -109,7 +112,7 @@ struct TilePages {
 
 // kLogits: the logits are stored as well (MapArgs::logits), a variant of its own so that the plain map keeps its code.
 template <typename Tag, int D, int G, int kWaves, bool kHalfPage, bool kLogits = false>
-__global__ __launch_bounds__(64 * kWaves, decode_waves_per_simd(G)) void split_kv_decode_map(
+__global__ __launch_bounds__(64 * kWaves, decode_waves_per_simd(G, kLogits)) void split_kv_decode_map(
     MapArgs a, const uint32_t* __restrict__ page_ids, const uint32_t* __restrict__ kv_splits,
     const uint32_t* __restrict__ req_slots, const uint16_t* __restrict__ q, const uint16_t* __restrict__ pages,
     const uint32_t* __restrict__ worker_cu) {
@@ -135,6 +138,7 @@ __global__ __launch_bounds__(64 * kWaves, decode_waves_per_simd(G)) void split_k
     __shared__ float merge_max[kWaves][G];
     __shared__ float merge_sum[kWaves][G];
     __shared__ __attribute__((aligned(16))) uint4 qb_lds[D / 32][64];
+    extern __shared__ __attribute__((aligned(16))) float4 logit_lds[];  // [wave][tile][head group's 16 bytes x 4]; kLogits
 
     // MFMA lane coordinates: row of A (token) and column of B / D (query row); 8-dim chunk of A
     // and B, token quad of D.
@@ -263,10 +267,27 @@ __global__ __launch_bounds__(64 * kWaves, decode_waves_per_simd(G)) void split_k
 
     float* my_p = p_lds[wave];
     float* my_alpha = alpha_lds[wave];
+    // The logits of whole tiles wait in LDS until there is no room for another of the wave's.  Stores that are scattered
+    // over the pass cost far more than their bytes (4 x 131072 tokens, 34 MB of logits beside 1.07 GB of K and V: 211 us
+    // with a store per tile, 199 us with one per 32 KB of a workgroup, 178 us per 96 KB, 160 us without them; the same
+    // stores to a line that stays in L2: 163 us), so they are kept back until the workgroup's share is read, or nearly.
+    constexpr uint32_t kUnits = 4 * G;  // 16-byte units of a tile
+    float4* const my_logits = kLogits ? logit_lds + (uint64_t)wave * a.logit_lds_tiles * kUnits : nullptr;
     float* logit_row = nullptr;
+    uint32_t logit_tiles = 0, logit_tile0 = 0;  // how many, and the first one's position; a wave's tiles are kWaves apart
     if constexpr (kLogits)
-        logit_row = a.logits + ((uint64_t)q_token * a.hq + (uint64_t)kv_head * G + (mt < (uint32_t)G ? mt : 0)) *
-                                   a.logits_stride;
+        logit_row = a.logits + logit_index(a.logits_stride, G, (uint64_t)q_token * a.walk.hkv + kv_head, 0, 0);
+    auto flush_logits = [&]() __attribute__((always_inline)) {
+        wave_lds_fence();
+        for (uint32_t i = lane; i < logit_tiles * kUnits; i += 64) {
+            const uint32_t n = i / kUnits, unit = i % kUnits;
+            const uint32_t first = logit_tile0 + n * (kWaves * kTileTokens);
+            const float4 l = my_logits[i];
+            if (first + kTileTokens <= a.logits_stride)
+                *reinterpret_cast<float4*>(logit_row + (uint64_t)first * G + unit * 4) = l;
+        }
+        logit_tiles = 0;
+    };
 
     // One 16-token tile.  `partial`: the tile holds tokens outside [kv_begin, kv_end).
     // `has_next`: another tile of this wave follows; its K and V are requested on the way, each
@@ -298,18 +319,18 @@ __global__ __launch_bounds__(64 * kWaves, decode_waves_per_simd(G)) void split_k
             m = fmaxf(m, v[r]);
         }
         if constexpr (kLogits) {
-            // 64 contiguous bytes per query row and tile; the tile that a request's end or a row's border cuts is
-            // stored token by token
-            if (mt < (uint32_t)G) {
-                float* dst = logit_row + base + mc * 4;
-                if (!partial && base + kTileTokens <= a.logits_stride) {
-                    *reinterpret_cast<float4*>(dst) = make_float4(v[0], v[1], v[2], v[3]);
-                } else {
+            if (!partial) {
+                if (mt < (uint32_t)G)
+                    my_logits[logit_tiles * kUnits + mc * G + mt] = make_float4(v[0], v[1], v[2], v[3]);
+                if (logit_tiles == 0) logit_tile0 = base;
+                if (++logit_tiles == a.logit_lds_tiles) flush_logits();
+            } else if (mt < (uint32_t)G) {
+                // a tile that a request's end or a row's border cuts, token by token
 #pragma unroll
-                    for (int r = 0; r < 4; ++r) {
-                        const uint32_t token = base + mc * 4 + r;
-                        if (token >= lo && token < hi && token < a.logits_stride) dst[r] = v[r];
-                    }
+                for (int r = 0; r < 4; ++r) {
+                    const uint32_t token = base + mc * 4 + r;
+                    if (token >= lo && token < hi && token < a.logits_stride)
+                        logit_row[logit_index(0, G, 0, token, mt)] = v[r];
                 }
             }
         }
@@ -424,6 +445,8 @@ __global__ __launch_bounds__(64 * kWaves, decode_waves_per_simd(G)) void split_k
         }
     }
 
+    if constexpr (kLogits) flush_logits();
+
     // ---- wave epilogue: fold the V token sub-lanes together, reduce the per-lane sums.
 #pragma unroll
     for (int h = 0; h < G; ++h)
@@ -478,16 +501,30 @@ __global__ __launch_bounds__(64 * kWaves, decode_waves_per_simd(G)) void split_k
 }
 
 
+// LDS of a workgroup without the logits', rounded up.
+constexpr uint32_t decode_lds_bytes(int d, int group) { return 2048 + 128 + 16 * group * d + 32 * group + 32 * d + 256; }
+constexpr uint32_t kLdsPerUnit = 163840;
+
 template <typename Tag, int D, int G, bool kLogits>
-inline void launch_decode_map_w(psi_hip_ctx* ctx, const Geometry& g, const MapArgs& a) {
+inline void launch_decode_map_w(psi_hip_ctx* ctx, const Geometry& g, const MapArgs& args) {
+    MapArgs a = args;
     const dim3 grid((a.worker_cu ? a.num_workers : a.num_total_kv_splits) * g.hkv);
+    uint32_t lds = 0;
+    if (kLogits) {
+        // All of a compute unit's LDS if the launch has a workgroup per unit (a balanced plan), else half of it, so that
+        // a second workgroup streams while the first one starts or ends.
+        const uint32_t resident = grid.x <= (uint32_t)ctx->num_cus ? 1 : 2;
+        const uint32_t tile = 4 * kTileTokens * G * 4;  // of the four waves
+        a.logit_lds_tiles = (kLdsPerUnit / resident - decode_lds_bytes(D, G)) / tile;
+        lds = a.logit_lds_tiles * tile;
+    }
     const uint16_t* q = reinterpret_cast<const uint16_t*>(a.q);
     const uint16_t* pages = reinterpret_cast<const uint16_t*>(a.kv_pages);
     if (g.tokens_per_page == 8)  // a tile spans two pages
-        hipLaunchKernelGGL((split_kv_decode_map<Tag, D, G, 4, true, kLogits>), grid, dim3(256), 0, ctx->stream, a,
+        hipLaunchKernelGGL((split_kv_decode_map<Tag, D, G, 4, true, kLogits>), grid, dim3(256), lds, ctx->stream, a,
                            a.walk.page_ids, a.kv_splits, a.req_slots, q, pages, a.worker_cu);
     else
-        hipLaunchKernelGGL((split_kv_decode_map<Tag, D, G, 4, false, kLogits>), grid, dim3(256), 0, ctx->stream, a,
+        hipLaunchKernelGGL((split_kv_decode_map<Tag, D, G, 4, false, kLogits>), grid, dim3(256), lds, ctx->stream, a,
                            a.walk.page_ids, a.kv_splits, a.req_slots, q, pages, a.worker_cu);
 }
 

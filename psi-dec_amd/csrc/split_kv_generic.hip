@@ -74,7 +74,8 @@ __global__ __launch_bounds__(64) void split_kv_map_generic(MapArgs a) {
                 dot += load_as_f32<Tag>(a.q, q_off + i) * load_as_f32<Tag>(a.kv_pages, k_off + i);
             logit2 = dot * a.scale_log2;
             if (a.logits != nullptr && slice == 0 && token < a.logits_stride)
-                a.logits[((uint64_t)q_token * a.hq + q_head) * a.logits_stride + token] = logit2;
+                a.logits[logit_index(a.logits_stride, a.group, (uint64_t)q_token * a.walk.hkv + kv_head, token, q_head % a.group)] =
+                    logit2;
             v_offsets[lane] = kv_line_offset(a.walk, req_slot, a.layer, token, 1, kv_head);
         }
         const float tile_max = wave_max(logit2);

@@ -129,11 +129,13 @@ class GQAKVObserveKernels:
 
 @dataclass
 class GQAKVEvictionPlan:
-    """The requests of an eviction on the device, and room for what they keep: one use at a time."""
+    """The requests of an eviction on the device, room for what they keep and the selection's scratch: one use at a
+    time."""
     requests: object
     num_reqs: int
     max_cached: int
     kept: object
+    scratch: object  # of a selection; None when it needs none
 
 
 class GQAKVEvictionKernels:
@@ -159,10 +161,15 @@ class GQAKVEvictionKernels:
         requests, most = np.empty(2 * len(rs), np.uint32), ctypes.c_uint32()
         L.check(L.load().psi_hip_kv_evict_plan(ctypes.byref(self._cfg), ctypes.byref(self._layout), _p(rs), _p(nc),
                                                len(rs), _p(requests), ctypes.byref(most)))
+        scratch = ctypes.c_uint64()
+        L.check(L.load().psi_hip_kv_select_scratch_bytes(ctypes.byref(self._cfg), len(rs), most.value,
+                                                         ctypes.byref(scratch)))
         with torch.cuda.stream(self.device.stream):
             kept = torch.empty((len(rs), self.config.num_kv_heads, self.budget), dtype=torch.int32,
                                device=self.device.torch_device)
-        return GQAKVEvictionPlan(_upload(self.device, requests), len(rs), most.value, kept)
+            buffer = (torch.empty(scratch.value, dtype=torch.uint8, device=self.device.torch_device) if scratch.value
+                      else None)
+        return GQAKVEvictionPlan(_upload(self.device, requests), len(rs), most.value, kept, buffer)
 
     def invoke_select(self, plan: GQAKVEvictionPlan, page_weights, page_ids, page_table_index: int):
         """The positions to keep, int32 [requests][KV heads][budget], ascending and padded with -1 (the 32-bit
@@ -171,7 +178,7 @@ class GQAKVEvictionKernels:
         L.check(self.device.lib.psi_hip_kv_select_kept(
             self.device.ctx, ctypes.byref(self._cfg), ctypes.byref(self._layout), _ptr(page_weights),
             _nbytes(page_weights), _ptr(page_ids), _ptr(plan.requests), plan.num_reqs, plan.max_cached, self.budget,
-            self.num_first, self.num_recent, _ptr(plan.kept), page_table_index))
+            self.num_first, self.num_recent, _ptr(plan.kept), _ptr(plan.scratch), _nbytes(plan.scratch), page_table_index))
         return plan.kept
 
     def invoke_compact(self, plan: GQAKVEvictionPlan, kept, kv_pages, page_weights, page_ids, page_table_index: int):

@@ -311,7 +311,9 @@ def test_selection(psi, device, values, budget, first, recent):
     assert np.array_equal(got, exp)
 
 
-@pytest.mark.parametrize("lens,hkv,page,ids", [([70001, 65536, 300], 2, 16, 1), ([40000], 8, 8, 4), ([9000, 33], 3, 5, 2)])
+@pytest.mark.parametrize("lens,hkv,page,ids", [([70001, 65536, 300], 2, 16, 1), ([40000], 8, 8, 4), ([9000, 33], 3, 5, 2),
+                                              ([16384, 4097, 8192], 2, 16, 1), ([16385, 24576, 24577, 8193, 5], 2, 16, 1),
+                                              ([20011, 12289], 2, 7, 1)])
 @pytest.mark.parametrize("values", ["softmax", "ties", "equal"])
 def test_selection_of_long_requests(psi, device, lens, hkv, page, ids, values):
     for budget, first, recent in ((256, 4, 32), (max(lens) // 2, 16, 100), (max(lens) - 1, 0, 0)):

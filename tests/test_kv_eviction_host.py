@@ -132,7 +132,8 @@ def test_null_arguments_are_refused_before_a_gpu_is_touched(psi):
                                                         None, None, 0, 1, 1, 1, 1) == L.ERR_INVALID_ARGUMENT
     assert lib.psi_hip_kv_observe_weights(None, c, y, None, 1, None, 0, None, None, 1, 1, None, 1, None, 0, None, 0, 1.0,
                                           0) == L.ERR_INVALID_ARGUMENT
-    assert lib.psi_hip_kv_select_kept(None, c, y, None, 0, None, None, 1, 1, 1, 0, 0, None, 0) == L.ERR_INVALID_ARGUMENT
+    assert lib.psi_hip_kv_select_kept(None, c, y, None, 0, None, None, 1, 1, 1, 0, 0, None, None, 0,
+                                      0) == L.ERR_INVALID_ARGUMENT
     assert lib.psi_hip_kv_compact(None, c, y, None, 0, None, 0, None, None, 1, 1, 1, None, 0) == L.ERR_INVALID_ARGUMENT
     assert b"must not be null" in lib.psi_hip_last_error()
 
