@@ -831,8 +831,8 @@ typedef struct psi_hip_kv_weights {
     float decay;                 /* 0 .. 1: what earlier steps' weights are multiplied by, 1 = plain sums */
 } psi_hip_kv_weights;
 
-/* Bytes of the logits that a step of up to num_total_tokens tokens stores, [tokens][num_q_heads][max_context_tokens
- * rounded up to 16] f32. */
+/* Bytes of the logits that a step of up to num_total_tokens tokens stores, f32 for every query head and position up
+ * to max_context_tokens rounded up to 64 (the layout is private to the library). */
 int psi_hip_split_kv_single_q_logits_bytes(const psi_hip_gqa_config* cfg, uint32_t num_total_tokens,
                                            uint32_t max_context_tokens, uint64_t* out_bytes);
 

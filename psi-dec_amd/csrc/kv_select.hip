@@ -284,13 +284,20 @@ __global__ __launch_bounds__(kSelectThreads) void select_chunk_kernel(SelectArgs
         // counters kBins - 1 - 2t and the one below: over the row, and over the chunks ahead
         uint32_t high = 0, low = 0, high_ahead = 0, low_ahead = 0;
         const uint32_t at = kBins - 2 - 2 * tid;
-        for (uint32_t c = 0; c < row_chunks; ++c) {
-            const uint2 v = *reinterpret_cast<const uint2*>(bins_of(kPass - 1, c) + at);
-            low += v.x;
-            high += v.y;
-            if (c < chunk) {
-                low_ahead += v.x;
-                high_ahead += v.y;
+        constexpr uint32_t kAhead = 16;  // chunks asked for at a time
+        for (uint32_t c0 = 0; c0 < row_chunks; c0 += kAhead) {
+            uint2 v[kAhead];
+#pragma unroll
+            for (uint32_t u = 0; u < kAhead; ++u)
+                v[u] = c0 + u < row_chunks ? *reinterpret_cast<const uint2*>(bins_of(kPass - 1, c0 + u) + at) : make_uint2(0, 0);
+#pragma unroll
+            for (uint32_t u = 0; u < kAhead; ++u) {
+                low += v[u].x;
+                high += v[u].y;
+                if (c0 + u < chunk) {
+                    low_ahead += v[u].x;
+                    high_ahead += v[u].y;
+                }
             }
         }
         find_bin(search, tid, high, low, st, kPass - 1);

@@ -31,15 +31,14 @@ constexpr uint32_t kFinishThreads = 512, kFinishWaves = kFinishThreads / 64;
 constexpr uint32_t kLseEntries = 512;  // (token, head) normalisers held in LDS at a time
 constexpr uint32_t kFewEntries = 8;    // up to this many (a decode step's heads) a thread holds the logits of all
 
-// log2 of the sum of exponentials of one (token, head) over its partial states, in every lane of the wave; +inf where
-// nothing contributes, so that the row's weights are zero.
-__device__ __forceinline__ float lse_of(const WeightsArgs& a, uint32_t token, uint32_t head, uint32_t lane) {
-    const uint32_t p0 = a.cu_kv_splits[token], p1 = a.cu_kv_splits[token + 1];
+// log2 of the sum of exponentials of one (token, head) over its partial states p0 .. p1, in every lane of the wave;
+// +inf where nothing contributes, so that the row's weights are zero.
+__device__ __forceinline__ float lse_of(const WeightsArgs& a, uint32_t p0, uint32_t p1, uint32_t head, uint32_t lane) {
     float m = -INFINITY, s = 0.0f;
     for (uint32_t p = p0 + lane; p < p1; p += 64) {
         const uint64_t r = (uint64_t)(a.row_index ? a.row_index[p] : p) * a.hq + head;
-        const float pm = a.part_max[r], next = fmaxf(m, pm);
-        if (pm > -INFINITY) s = s * exp2f(m - next) + a.part_sum[r] * exp2f(pm - next);
+        const float pm = a.part_max[r], ps = a.part_sum[r], next = fmaxf(m, pm);
+        if (pm > -INFINITY) s = s * exp2f(m - next) + ps * exp2f(pm - next);
         m = next;
     }
 #pragma unroll
@@ -64,11 +63,16 @@ __device__ __forceinline__ void accumulate_row(const WeightsArgs& a, uint32_t sp
     if (split >= num_splits) return;
     const uint32_t token = a.kv_splits[split * 3], begin = a.kv_splits[split * 3 + 1], row_end = a.kv_splits[split * 3 + 2];
     if (token >= num_tokens) return;
-    const uint32_t slot = a.req_slots[token];
-    if (token + 1 < num_tokens && a.req_slots[token + 1] == slot) return;
-    uint32_t first = token;
-    while (first > 0 && a.req_slots[first - 1] == slot) --first;
-    const uint32_t held = a.flat_token_indices[first], own = a.flat_token_indices[token];
+    // asked for together: whatever depends on the token alone
+    const uint32_t before = token > 0 ? token - 1 : 0, after = min(token + 1, num_tokens - 1);
+    const uint32_t slot = a.req_slots[token], slot_before = a.req_slots[before], slot_after = a.req_slots[after];
+    const uint32_t own = a.flat_token_indices[token], p0 = a.cu_kv_splits[token], p1 = a.cu_kv_splits[token + 1];
+    if (after != token && slot_after == slot) return;
+    uint32_t first = token, held = own;
+    if (before != token && slot_before == slot) {
+        for (first = before; first > 0 && a.req_slots[first - 1] == slot;) --first;
+        held = a.flat_token_indices[first];
+    }
     const uint32_t end = min(row_end, a.max_context);
     if (threadIdx.x == 0 && row_end > end) report_cache_range(a.status);
     const uint32_t* row = table_row(a.v, slot, layer);
@@ -77,17 +81,19 @@ __device__ __forceinline__ void accumulate_row(const WeightsArgs& a, uint32_t sp
     const bool vector = a.v.log2_page < 32 && a.v.log2_page >= 2 && reinterpret_cast<uintptr_t>(a.page_weights) % 16 == 0;
 
     // the accumulators of positions p .. p + 3, from `sum`; `first_turn`: on top of what counts already
-    auto add = [&](uint32_t p, const float (&sum)[4], uint32_t page, bool first_turn) {
-        if (vector && p >= begin && p + 4 <= end) {
+    auto whole = [&](uint32_t p) { return vector && p >= begin && p + 4 <= end; };
+    auto slot_of = [&](uint32_t p, uint32_t page) {
+        return reinterpret_cast<float4*>(a.page_weights + weight_index(a.v, page, kv_head, page_place(a.v, p)));
+    };
+    auto add = [&](uint32_t p, const float (&sum)[4], uint32_t page, float4 old, bool first_turn) {
+        if (whole(p)) {
             if (page == kNoPage) {
                 report_cache_range(a.status);
                 return;
             }
-            float4* acc = reinterpret_cast<float4*>(a.page_weights + weight_index(a.v, page, kv_head, page_place(a.v, p)));
-            const float4 old = *acc;
             auto base = [&](float x, uint32_t at) { return !first_turn ? x : at < held ? a.decay * x : 0.0f; };
-            *acc = make_float4(base(old.x, p) + sum[0], base(old.y, p + 1) + sum[1], base(old.z, p + 2) + sum[2],
-                               base(old.w, p + 3) + sum[3]);
+            *slot_of(p, page) = make_float4(base(old.x, p) + sum[0], base(old.y, p + 1) + sum[1],
+                                            base(old.z, p + 2) + sum[2], base(old.w, p + 3) + sum[3]);
             return;
         }
 #pragma unroll
@@ -109,15 +115,17 @@ __device__ __forceinline__ void accumulate_row(const WeightsArgs& a, uint32_t sp
         const float* token_logits = a.logits + logit_index(a.logits_stride, a.group, (uint64_t)token * a.v.hkv + kv_head, 0, 0);
         float4 l[kFewEntries];
         uint32_t page = kNoPage;
+        float4 old = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
         auto fetch = [&](uint32_t p) {
 #pragma unroll
             for (uint32_t e = 0; e < kFewEntries; ++e)
-                if (e < entries) l[e] = *reinterpret_cast<const float4*>(token_logits + (uint64_t)p * a.group + e * 4);
+                if (e < entries) l[e] = *reinterpret_cast<const float4*>(token_logits + logit_index(0, a.group, 0, p, e));
             page = page_of(a.v, row, p, a.v.num_weight_pages);
+            if (whole(p) && page != kNoPage) old = *slot_of(p, page);
         };
         if (start < end) fetch(start);
         if (wave < entries) {
-            const float x = lse_of(a, token, kv_head * a.group + wave, lane);
+            const float x = lse_of(a, p0, p1, kv_head * a.group + wave, lane);
             if (lane == 0) lse[wave] = x;
         }
         __syncthreads();
@@ -131,7 +139,7 @@ __device__ __forceinline__ void accumulate_row(const WeightsArgs& a, uint32_t sp
 #pragma unroll
                 for (int i = 0; i < 4; ++i) sum[i] += p + i <= own ? __builtin_amdgcn_exp2f(x[i] - lse[e]) : 0.0f;
             }
-            add(p, sum, page, true);
+            add(p, sum, page, old, true);
         }
         return;
     }
@@ -139,7 +147,8 @@ __device__ __forceinline__ void accumulate_row(const WeightsArgs& a, uint32_t sp
         const uint32_t count = min(kLseEntries, entries - base);
         if (base > 0) __syncthreads();
         for (uint32_t e = wave; e < count; e += kFinishWaves) {
-            const float x = lse_of(a, first + (base + e) / a.group, kv_head * a.group + (base + e) % a.group, lane);
+            const uint32_t t = first + (base + e) / a.group;
+            const float x = lse_of(a, a.cu_kv_splits[t], a.cu_kv_splits[t + 1], kv_head * a.group + (base + e) % a.group, lane);
             if (lane == 0) lse[e] = x;
         }
         __syncthreads();
@@ -159,7 +168,8 @@ __device__ __forceinline__ void accumulate_row(const WeightsArgs& a, uint32_t sp
                     ++t;
                 }
             }
-            add(p, sum, page, base == 0);
+            const float4 old = whole(p) && page != kNoPage ? *slot_of(p, page) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            add(p, sum, page, old, base == 0);
         }
     }
 }
@@ -197,7 +207,7 @@ __global__ __launch_bounds__(kFinishThreads) void accumulate_kernel(WeightsArgs 
     accumulate_row(w, blockIdx.x / w.v.hkv, blockIdx.x % w.v.hkv, lse);
 }
 
-static uint64_t logits_stride(uint32_t max_context_tokens) { return ((uint64_t)max_context_tokens + 15) / 16 * 16; }
+static uint64_t logits_stride(uint32_t max_context_tokens) { return ((uint64_t)max_context_tokens + 63) / 64 * 64; }
 
 }  // namespace psi
 

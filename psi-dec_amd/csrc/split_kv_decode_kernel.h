@@ -138,7 +138,7 @@ __global__ __launch_bounds__(64 * kWaves, decode_waves_per_simd(G, kLogits)) voi
     __shared__ float merge_max[kWaves][G];
     __shared__ float merge_sum[kWaves][G];
     __shared__ __attribute__((aligned(16))) uint4 qb_lds[D / 32][64];
-    extern __shared__ __attribute__((aligned(16))) float4 logit_lds[];  // [wave][tile][head group's 16 bytes x 4]; kLogits
+    extern __shared__ __attribute__((aligned(16))) float4 logit_lds[];  // [wave][tile][head][four positions]; kLogits
 
     // MFMA lane coordinates: row of A (token) and column of B / D (query row); 8-dim chunk of A
     // and B, token quad of D.
@@ -271,7 +271,7 @@ __global__ __launch_bounds__(64 * kWaves, decode_waves_per_simd(G, kLogits)) voi
     // over the pass cost far more than their bytes (4 x 131072 tokens, 34 MB of logits beside 1.07 GB of K and V: 211 us
     // with a store per tile, 199 us with one per 32 KB of a workgroup, 178 us per 96 KB, 160 us without them; the same
     // stores to a line that stays in L2: 163 us), so they are kept back until the workgroup's share is read, or nearly.
-    constexpr uint32_t kUnits = 4 * G;  // 16-byte units of a tile
+    constexpr uint32_t kUnits = 4 * G;  // 16-byte units of a tile, [head][four positions]
     float4* const my_logits = kLogits ? logit_lds + (uint64_t)wave * a.logit_lds_tiles * kUnits : nullptr;
     float* logit_row = nullptr;
     uint32_t logit_tiles = 0, logit_tile0 = 0;  // how many, and the first one's position; a wave's tiles are kWaves apart
@@ -284,7 +284,7 @@ __global__ __launch_bounds__(64 * kWaves, decode_waves_per_simd(G, kLogits)) voi
             const uint32_t first = logit_tile0 + n * (kWaves * kTileTokens);
             const float4 l = my_logits[i];
             if (first + kTileTokens <= a.logits_stride)
-                *reinterpret_cast<float4*>(logit_row + (uint64_t)first * G + unit * 4) = l;
+                *reinterpret_cast<float4*>(logit_row + logit_index(0, G, 0, first + unit % 4 * 4, unit / 4)) = l;
         }
         logit_tiles = 0;
     };
@@ -321,7 +321,7 @@ __global__ __launch_bounds__(64 * kWaves, decode_waves_per_simd(G, kLogits)) voi
         if constexpr (kLogits) {
             if (!partial) {
                 if (mt < (uint32_t)G)
-                    my_logits[logit_tiles * kUnits + mc * G + mt] = make_float4(v[0], v[1], v[2], v[3]);
+                    my_logits[logit_tiles * kUnits + mt * 4 + mc] = make_float4(v[0], v[1], v[2], v[3]);
                 if (logit_tiles == 0) logit_tile0 = base;
                 if (++logit_tiles == a.logit_lds_tiles) flush_logits();
             } else if (mt < (uint32_t)G) {

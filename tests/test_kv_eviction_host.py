@@ -40,10 +40,10 @@ def test_page_weights_bytes(psi):
             L.check(L.load().psi_hip_kv_page_weights_bytes(ctypes.byref(cfg), pages, ctypes.byref(out)))
 
 
-def test_logits_bytes_round_the_context_up_to_a_tile(psi):
+def test_logits_bytes_round_the_context_up_to_a_block(psi):
     L, cfg, out = psi._lib, _config(psi).struct(), ctypes.c_uint64()
     L.check(L.load().psi_hip_split_kv_single_q_logits_bytes(ctypes.byref(cfg), 3, 17, ctypes.byref(out)))
-    assert out.value == 3 * 24 * 32 * 4
+    assert out.value == 3 * 24 * 64 * 4
     with pytest.raises(psi.PsiHipError, match="need tokens and a context"):
         L.check(L.load().psi_hip_split_kv_single_q_logits_bytes(ctypes.byref(cfg), 3, 0, ctypes.byref(out)))
 
