@@ -9,6 +9,8 @@
 
 namespace psi {
 
+typedef uint32_t unit_u32x4 __attribute__((ext_vector_type(4)));
+
 struct CompactArgs {
     CacheView v;
     void* pages;
@@ -18,71 +20,123 @@ struct CompactArgs {
     uint32_t* status;
     uint32_t max_cached, budget;
     uint32_t line_units, slice_units, num_slices;  // units of a line, of a slice; slices of a line
+    uint32_t num_reqs, group_stride;               // group_stride: workgroups between two slices of a line
 };
 
-constexpr uint32_t kCompactThreads = 1024;
-constexpr int kCompactUnroll = 4;
+// The runs of one (request, KV head, slice): a workgroup takes `per_step` lines at a time, a unit a lane, kUnroll
+// steps a run.  What a run's lines need is asked for ahead, a link of the chain per run: the kept positions two runs
+// ahead, the page IDs one run ahead, then the lines, so that a run waits for memory once.  Entries that move nothing read
+// the first unit of the array in place of a line, so that the loads of a run stand without branches between them.
+template <int kUnroll, typename Unit, typename Index>
+__device__ __forceinline__ void move_runs(const CompactArgs& a, const uint32_t* kept, const uint32_t* table, uint32_t n,
+                                          uint32_t num_pages, Unit* data, uint32_t my_line, uint32_t per_step, bool in_line,
+                                          Index index) {
+    const uint32_t per_run = per_step * kUnroll;
+    uint32_t src[kUnroll], src_next[kUnroll], from[kUnroll], to[kUnroll];
+    auto entry = [&](uint32_t base, int u) -> uint32_t { return base + u * per_step + my_line; };
+    auto fetch_kept = [&](uint32_t base, uint32_t (&out)[kUnroll]) {
+#pragma unroll
+        for (int u = 0; u < kUnroll; ++u) {
+            const uint32_t i = entry(base, u);
+            const bool there = in_line && i < a.budget;
+            const uint32_t k = kept[there ? i : 0];
+            out[u] = there ? k : i;  // an entry that stays where it is moves nothing
+        }
+    };
+    auto fetch_pages = [&](uint32_t base, const uint32_t (&at)[kUnroll]) {
+#pragma unroll
+        for (int u = 0; u < kUnroll; ++u) {
+            const uint32_t i = entry(base, u);
+            const bool moves = at[u] > i && at[u] < n;  // (n's positions have entries in the table)
+            from[u] = table[moves ? page_index(a.v, at[u]) : 0];
+            to[u] = table[moves ? page_index(a.v, i) : 0];
+            if (!moves || from[u] >= num_pages || to[u] >= num_pages) from[u] = to[u] = kNoPage;
+        }
+    };
+    fetch_kept(0, src);
+    fetch_kept(per_run, src_next);
+    fetch_pages(0, src);
+    for (uint32_t base = 0; base < a.budget; base += per_run) {
+        Unit held[kUnroll];
+        uint64_t target[kUnroll];
+        uint32_t moves = 0;
+#pragma unroll
+        for (int u = 0; u < kUnroll; ++u) {
+            const uint32_t i = entry(base, u);
+            const bool found = from[u] != kNoPage;
+            // beyond the cached tokens or the arena, or not ascending: nothing is moved for this entry
+            if (!found && src[u] != i) report_cache_range(a.status);
+            held[u] = __builtin_nontemporal_load(data + (found ? index(from[u], src[u]) : 0));
+            target[u] = index(to[u], i);
+            moves |= (found ? 1u : 0u) << u;
+        }
+        fetch_pages(base + per_run, src_next);
+#pragma unroll
+        for (int u = 0; u < kUnroll; ++u) src[u] = src_next[u];
+        fetch_kept(base + 2 * per_run, src_next);
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // the run has been read ...
+        __syncthreads();                                  // ... by every wave before any of it is written
+#pragma unroll
+        for (int u = 0; u < kUnroll; ++u)
+            if (moves >> u & 1) data[target[u]] = held[u];
+    }
+}
 
-// One workgroup per (request, KV head, slice of K | slice of V | accumulators); slice_units divides kCompactThreads.
-template <typename Unit>
-__global__ __launch_bounds__(kCompactThreads) void compact_kernel(CompactArgs a) {
-    const uint32_t parts = 2 * a.num_slices + (a.page_weights != nullptr ? 1u : 0u);
-    const uint32_t part = blockIdx.x % parts, kv_head = blockIdx.x / parts % a.v.hkv, req = blockIdx.x / parts / a.v.hkv;
-    const uint32_t slot = a.requests[req * kRequestWords], n = min(min(a.requests[req * kRequestWords + 1], a.max_cached), a.v.positions);
+// One workgroup per (slice, request, KV head, K | V), then one per (request, KV head) for the accumulators; slice_units
+// divides kThreads.  The slices of a line are a multiple of eight workgroups apart, so that they go to one XCD and share
+// in its L2 the lines of memory that a slice of less than 128 bytes reads a part of.
+template <typename Unit, int kThreads, int kUnroll>
+__global__ __launch_bounds__(kThreads) void compact_kernel(CompactArgs a) {
+    const uint32_t line_groups = a.group_stride * a.num_slices;
+    const bool is_weights = blockIdx.x >= line_groups;
+    const uint32_t pair = is_weights ? (blockIdx.x - line_groups) * 2 : blockIdx.x % a.group_stride;
+    const uint32_t kind = pair % 2, kv_head = pair / 2 % a.v.hkv, req = pair / 2 / a.v.hkv;
+    if (req >= a.num_reqs) return;
+    const uint32_t slot = a.requests[req * kRequestWords];
+    const uint32_t n = min(min(a.requests[req * kRequestWords + 1], a.max_cached), a.v.positions);
     if (n <= a.budget) return;  // everything is kept where it is
     if (slot >= a.v.num_slots) {
         report_cache_range(a.status);
         return;
     }
     const uint32_t* kept = a.kept + ((uint64_t)req * a.v.hkv + kv_head) * a.budget;
-    const uint32_t* row = table_row(a.v, slot, a.v.layer);
-    const bool is_weights = part == 2 * a.num_slices;
-    const uint32_t kind = part / a.num_slices, unit0 = part % a.num_slices * a.slice_units;
-    const uint32_t width = is_weights ? 1 : a.slice_units, per_round = kCompactThreads / width;
-    const uint32_t my_line = threadIdx.x / width, my_unit = unit0 + threadIdx.x % width;
-    const bool in_line = is_weights || my_unit < a.line_units;
-    const uint32_t limit = is_weights ? a.v.num_weight_pages : a.v.num_pages;
-    Unit* lines = static_cast<Unit*>(a.pages);
-    auto unit_index = [&](uint32_t page, uint32_t place) -> uint64_t {
-        const uint64_t line = ((uint64_t)page * 2 + kind) * a.v.hkv * a.v.tokens_per_page +
-                              (uint64_t)kv_head * a.v.tokens_per_page + place;
-        return line * a.line_units + my_unit;
-    };
-    for (uint32_t base = 0; base < a.budget; base += per_round * kCompactUnroll) {
-        Unit held[kCompactUnroll] = {};
-        float weight[kCompactUnroll] = {};
-        uint32_t to_page[kCompactUnroll];
-        uint32_t i[kCompactUnroll];
-#pragma unroll
-        for (int u = 0; u < kCompactUnroll; ++u) {
-            i[u] = base + u * per_round + my_line;
-            to_page[u] = kNoPage;
-            if (!in_line || i[u] >= a.budget) continue;
-            const uint32_t src = kept[i[u]];
-            if (src == i[u]) continue;
-            if (src < i[u] || src >= n) {  // no ascending choice among the cached tokens: nothing is moved for it
-                report_cache_range(a.status);
-                continue;
-            }
-            const uint32_t from_page = page_of(a.v, row, src, limit);
-            to_page[u] = page_of(a.v, row, i[u], limit);
-            if (from_page == kNoPage || to_page[u] == kNoPage) {
-                report_cache_range(a.status);
-                to_page[u] = kNoPage;
-                continue;
-            }
-            if (is_weights) weight[u] = a.page_weights[weight_index(a.v, from_page, kv_head, page_place(a.v, src))];
-            else held[u] = lines[unit_index(from_page, page_place(a.v, src))];
-        }
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // the run has been read ...
-        __syncthreads();                                  // ... by every wave before any of it is written
-#pragma unroll
-        for (int u = 0; u < kCompactUnroll; ++u) {
-            if (to_page[u] == kNoPage) continue;
-            if (is_weights) a.page_weights[weight_index(a.v, to_page[u], kv_head, page_place(a.v, i[u]))] = weight[u];
-            else lines[unit_index(to_page[u], page_place(a.v, i[u]))] = held[u];
-        }
+    const uint32_t* table = table_row(a.v, slot, a.v.layer);
+    if (is_weights) {
+        move_runs<kUnroll>(a, kept, table, n, a.v.num_weight_pages, reinterpret_cast<uint32_t*>(a.page_weights), threadIdx.x,
+                           kThreads, true, [&](uint32_t page, uint32_t position) {
+                               return weight_index(a.v, page, kv_head, page_place(a.v, position));
+                           });
+        return;
     }
+    const uint32_t my_unit = blockIdx.x / a.group_stride * a.slice_units + threadIdx.x % a.slice_units;
+    move_runs<kUnroll>(a, kept, table, n, a.v.num_pages, static_cast<Unit*>(a.pages), threadIdx.x / a.slice_units,
+                       kThreads / a.slice_units, my_unit < a.line_units, [&](uint32_t page, uint32_t position) -> uint64_t {
+                           const uint64_t line = (((uint64_t)page * 2 + kind) * a.v.hkv + kv_head) * a.v.tokens_per_page +
+                                                 page_place(a.v, position);
+                           return line * a.line_units + my_unit;
+                       });
+}
+
+// Slices of a line: down to 128 bytes until there are four workgroups to a compute unit (32 requests of 1k-8k tokens cut
+// to 1024, 4 heads of 256: 86 us with whole lines, 48 us with 128 bytes, which is 5.4 TB/s read and written); where that
+// leaves compute units without one, down to 64 bytes (one request of 61001 tokens cut to 30000, 4 heads of 256: 206 us
+// with 128 bytes, 175 us with 64, 168 us with 32; four of 16000 cut to 8000, 8 heads of 128: 74, 69 and 118 us).
+inline uint32_t compact_slices(uint64_t pairs, uint32_t line_bytes) {
+    uint32_t slices = 1;
+    auto can_halve = [&](uint32_t least) { return line_bytes / (2 * slices) >= least; };
+    while ((slices * pairs < 1024 && can_halve(128)) || (slices * pairs < 256 && can_halve(64))) slices *= 2;
+    return slices;
+}
+
+template <typename Unit>
+static void launch_compact(psi_hip_ctx* ctx, const CompactArgs& a, uint32_t grid) {
+    // Many workgroups: short runs, several to a compute unit (55 us with four units a lane, 48 us with two on the 32
+    // requests above).  Few: long runs, which a wait for memory each costs less of (one of 61001: 378 us with 512 threads
+    // and two units, 216 us with 1024 and four, in 128-byte slices).
+    if (grid >= 512)
+        hipLaunchKernelGGL((compact_kernel<Unit, 512, 2>), dim3(grid), dim3(512), 0, ctx->stream, a);
+    else
+        hipLaunchKernelGGL((compact_kernel<Unit, 1024, 4>), dim3(grid), dim3(1024), 0, ctx->stream, a);
 }
 
 }  // namespace psi
@@ -119,19 +173,20 @@ extern "C" int psi_hip_kv_compact(psi_hip_ctx* ctx, const psi_hip_gqa_config* cf
     const uint32_t line_bytes = g.d * g.elem;
     const uint32_t unit = (line_bytes | (uint32_t)(reinterpret_cast<uintptr_t>(kv_pages) & 15)) % 16 == 0 ? 16 : g.elem;
     a.line_units = line_bytes / unit;
-    // 128 bytes of a line to a workgroup
-    const uint32_t most = 128 / unit;
+    const uint64_t pairs = (uint64_t)num_reqs * g.hkv * 2, stride = (pairs + 7) / 8 * 8;
+    const uint32_t slices = compact_slices(pairs, line_bytes);
     a.slice_units = 1;
-    while (a.slice_units < most && a.slice_units < a.line_units) a.slice_units *= 2;
+    while (a.slice_units < 512 && a.slice_units * slices < a.line_units) a.slice_units *= 2;
     a.num_slices = (a.line_units + a.slice_units - 1) / a.slice_units;
-    const uint64_t grid = (uint64_t)num_reqs * g.hkv * (2 * a.num_slices + (page_weights != nullptr ? 1 : 0));
+    a.num_reqs = num_reqs;
+    const uint64_t grid = stride * a.num_slices + (page_weights != nullptr ? pairs / 2 : 0);
     PSI_REQUIRE(grid <= 0x7fffffffull, "too many requests in one compaction");
     DeviceGuard guard(ctx->device);
     LaunchScope scope(ctx, "kv_compact");
-    const dim3 blocks((uint32_t)grid), threads(kCompactThreads);
-    if (unit == 16) hipLaunchKernelGGL(compact_kernel<uint4>, blocks, threads, 0, ctx->stream, a);
-    else if (unit == 4) hipLaunchKernelGGL(compact_kernel<uint32_t>, blocks, threads, 0, ctx->stream, a);
-    else hipLaunchKernelGGL(compact_kernel<uint16_t>, blocks, threads, 0, ctx->stream, a);
+    a.group_stride = (uint32_t)stride;
+    if (unit == 16) launch_compact<unit_u32x4>(ctx, a, (uint32_t)grid);
+    else if (unit == 4) launch_compact<uint32_t>(ctx, a, (uint32_t)grid);
+    else launch_compact<uint16_t>(ctx, a, (uint32_t)grid);
     PSI_HIP_CHECK(hipGetLastError());
     return PSI_HIP_OK;
 }
