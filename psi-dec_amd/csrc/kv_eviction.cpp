@@ -89,9 +89,10 @@ extern "C" int psi_hip_kv_page_weights_bytes(const psi_hip_gqa_config* cfg, uint
     return PSI_HIP_OK;
 }
 
-// Rows per KV head that a plan aims at, over all windows: two workgroups of each kernel per compute unit.
-constexpr uint32_t kObserveWorkgroups = 512;
-constexpr uint32_t kObserveRowTokens = 256;  // rows are cut at multiples of this
+// Workgroups that a plan aims at, over all windows and KV heads: one per compute unit, as a workgroup fills it (two
+// rounds of them take 80 us for 66 with 8 prompts of 1k-8k, 150 for 127 with one of 65536).
+constexpr uint32_t kObserveWorkgroups = 256;
+constexpr uint32_t kObserveRowTokens = 64;  // rows are cut at multiples of this (256: 18 us for 13 with one prompt of 777)
 
 extern "C" int psi_hip_kv_observe_plan(const psi_hip_gqa_config* cfg, const psi_hip_page_table_layout* layout,
                                        const uint32_t* req_slots, const uint32_t* token_indices,
@@ -119,9 +120,16 @@ extern "C" int psi_hip_kv_observe_plan(const psi_hip_gqa_config* cfg, const psi_
         total += context;
         max_window = std::max(max_window, window);
     }
-    const uint64_t aim = std::max<uint64_t>(1, kObserveWorkgroups / g.hkv);
-    uint64_t part = (total + aim - 1) / aim;
-    part = (part + kObserveRowTokens - 1) / kObserveRowTokens * kObserveRowTokens;
+    // the shortest rows of which no more than that many workgroups come, or one row to a window
+    const uint64_t aim = std::max<uint64_t>(std::max<uint64_t>(1, kObserveWorkgroups / g.hkv), num_reqs);
+    uint64_t part = ((total + aim - 1) / aim + kObserveRowTokens - 1) / kObserveRowTokens * kObserveRowTokens;
+    auto rows_at = [&](uint64_t tokens) {
+        uint64_t rows = 0;
+        for (uint32_t r = 0; r < num_reqs; ++r)
+            rows += ((uint64_t)token_indices[r] + (cu_tokens[r + 1] - cu_tokens[r]) + tokens - 1) / tokens;
+        return rows;
+    };
+    while (rows_at(part) > aim) part += std::max<uint64_t>(kObserveRowTokens, part / 16 / kObserveRowTokens * kObserveRowTokens);
     uint64_t n = 0;
     for (uint32_t r = 0; r < num_reqs; ++r) {
         const uint64_t context = (uint64_t)token_indices[r] + (cu_tokens[r + 1] - cu_tokens[r]);

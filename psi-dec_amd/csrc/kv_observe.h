@@ -23,7 +23,7 @@ struct ObserveArgs {
     uint32_t hq, group;
     float scale_log2, decay;
     float2* stats;  // [row][kv head][token in window][head of the group]: maximum (log2 domain) and sum
-    float* lse;     // [query row][q head], shape-generic kernels only
+    float* lse;     // [query row][q head]; null in the second pass: joined there
     float* page_weights;
     uint32_t* status;
 };
@@ -38,7 +38,7 @@ struct ObserveRow {
 };
 __device__ __forceinline__ ObserveRow load_row(const ObserveArgs& a, uint32_t row) {
     ObserveRow r;
-    const uint32_t w = a.rows[row * 3];
+    const uint32_t w = a.rows[(uint64_t)row * 3];
     r.live = w < a.num_windows && a.windows[(uint64_t)w * kWindowWords] < a.v.num_slots;
     const uint32_t* win = a.windows + (uint64_t)(r.live ? w : 0) * kWindowWords;
     r.slot = win[0];
@@ -48,8 +48,8 @@ __device__ __forceinline__ ObserveRow load_row(const ObserveArgs& a, uint32_t ro
     r.held = win[4];
     r.row_begin = win[5];
     r.row_end = min(win[6], a.num_rows);
-    r.begin = a.rows[row * 3 + 1];
-    r.end = min(min(a.rows[row * 3 + 2], r.position + r.num_q), a.v.positions);
+    r.begin = a.rows[(uint64_t)row * 3 + 1];
+    r.end = min(min(a.rows[(uint64_t)row * 3 + 2], r.position + r.num_q), a.v.positions);
     return r;
 }
 
@@ -57,23 +57,32 @@ __device__ __forceinline__ uint64_t stat_index(const ObserveArgs& a, uint32_t ro
     return ((uint64_t)row * a.v.hkv + kv_head) * a.max_window * a.group + column;
 }
 
-// The normaliser of one column from its window's rows; +inf where no key contributes, so that its weights are zero.
-__device__ __forceinline__ float join_column(const ObserveArgs& a, const ObserveRow& r, uint32_t kv_head, uint32_t column) {
-    constexpr int kAhead = 8;
-    float m = kEmptyMax, s = 0.0f;
-    for (uint32_t row = r.row_begin; row < r.row_end; row += kAhead) {
+// (m, s) joined with another state of the same column.
+__device__ __forceinline__ void join_states(float2 part, float* m, float* s) {
+    const float next = fmaxf(*m, part.x);
+    *s = *s * exp2f(*m - next) + part.y * exp2f(part.x - next);
+    *m = next;
+}
+// +inf where no key contributes, so that the column's weights are zero.
+__device__ __forceinline__ float lse_of_state(float m, float s) { return s == 0.0f ? INFINITY : m + log2f(s); }
+// The states of one column over rows first, first + step, ... before row_end.
+__device__ __forceinline__ void join_rows(const ObserveArgs& a, uint32_t first, uint32_t row_end, uint32_t step,
+                                          uint32_t kv_head, uint32_t column, float* m, float* s) {
+    constexpr uint32_t kAhead = 8;
+    for (uint32_t row = first; row < row_end; row += kAhead * step) {
         float2 part[kAhead];
 #pragma unroll
-        for (int u = 0; u < kAhead; ++u)
-            part[u] = row + u < r.row_end ? a.stats[stat_index(a, row + u, kv_head, column)] : make_float2(kEmptyMax, 0.0f);
+        for (uint32_t u = 0; u < kAhead; ++u)
+            part[u] = row + u * step < row_end ? a.stats[stat_index(a, row + u * step, kv_head, column)]
+                                               : make_float2(kEmptyMax, 0.0f);
 #pragma unroll
-        for (int u = 0; u < kAhead; ++u) {
-            const float next = fmaxf(m, part[u].x);
-            s = s * exp2f(m - next) + part[u].y * exp2f(part[u].x - next);
-            m = next;
-        }
+        for (uint32_t u = 0; u < kAhead; ++u) join_states(part[u], m, s);
     }
-    return s == 0.0f ? INFINITY : m + log2f(s);
+}
+__device__ __forceinline__ float join_column(const ObserveArgs& a, const ObserveRow& r, uint32_t kv_head, uint32_t column) {
+    float m = kEmptyMax, s = 0.0f;
+    join_rows(a, r.row_begin, r.row_end, 1, kv_head, column, &m, &s);
+    return lse_of_state(m, s);
 }
 
 // First weights of a position in this call: on top of what counts already.  Later ones: on top of the first.
@@ -87,6 +96,9 @@ __device__ __forceinline__ void add_weight(const ObserveArgs& a, const ObserveRo
     float* acc = a.page_weights + weight_index(a.v, page, kv_head, page_place(a.v, p));
     *acc = (!first ? *acc : p < r.held ? a.decay * *acc : 0.0f) + sum;
 }
+
+// The normalisers of all query rows and heads into a.lse, between the two passes.
+void launch_observe_join(psi_hip_ctx* ctx, const ObserveArgs& a);
 
 // Matrix-core kernels (kv_observe_kernel.h), one translation unit per element type; head_dim 128 or 256.
 void launch_observe_bf16(psi_hip_ctx* ctx, const ObserveArgs& a);

@@ -45,19 +45,29 @@ __global__ __launch_bounds__(64) void observe_stats_generic(ObserveArgs a) {
     }
 }
 
-// lse of every query row and head from its window's rows.
-__global__ __launch_bounds__(256) void observe_join(ObserveArgs a) {
+// One workgroup per (window, 32 (query row, head) items): eight threads share the rows of an item.
+constexpr uint32_t kJoinItems = 32, kJoinParts = 8;
+__global__ __launch_bounds__(kJoinItems * kJoinParts) void observe_join(ObserveArgs a) {
     const uint32_t* win = a.windows + (uint64_t)blockIdx.y * kWindowWords;
-    ObserveRow r;
-    r.q_begin = min(win[1], a.num_q_tokens);
-    r.num_q = min(min(win[2], a.max_window), a.num_q_tokens - r.q_begin);
-    r.row_begin = win[5];
-    r.row_end = min(win[6], a.num_rows);
-    const uint32_t item = blockIdx.x * 256 + threadIdx.x;
-    if (item >= r.num_q * a.hq) return;
-    const uint32_t head = item % a.hq;
-    a.lse[(uint64_t)r.q_begin * a.hq + item] =
-        join_column(a, r, head / a.group, item / a.hq * a.group + head % a.group);
+    const uint32_t q_begin = min(win[1], a.num_q_tokens), num_q = min(min(win[2], a.max_window), a.num_q_tokens - q_begin);
+    const uint32_t row_begin = win[5], row_end = min(win[6], a.num_rows);
+    const uint32_t item = blockIdx.x * kJoinItems + threadIdx.x % kJoinItems, part = threadIdx.x / kJoinItems;
+    __shared__ float2 parts[kJoinParts][kJoinItems];
+    // items in the order of the statistics: KV head, token, head of the group
+    const uint32_t columns = num_q * a.group, kv_head = item / max(columns, 1u), column = item % max(columns, 1u);
+    const bool live = item < columns * a.v.hkv;
+    float m = kEmptyMax, s = 0.0f;
+    if (live) join_rows(a, row_begin + part, row_end, kJoinParts, kv_head, column, &m, &s);
+    parts[part][threadIdx.x % kJoinItems] = make_float2(m, s);
+    __syncthreads();
+    if (part != 0 || !live) return;
+    for (uint32_t i = 1; i < kJoinParts; ++i) join_states(parts[i][threadIdx.x], &m, &s);
+    a.lse[(uint64_t)(q_begin + column / a.group) * a.hq + kv_head * a.group + column % a.group] = lse_of_state(m, s);
+}
+
+void launch_observe_join(psi_hip_ctx* ctx, const ObserveArgs& a) {
+    const dim3 grid((a.max_window * a.hq + kJoinItems - 1) / kJoinItems, a.num_windows);
+    hipLaunchKernelGGL(observe_join, grid, dim3(kJoinItems * kJoinParts), 0, ctx->stream, a);
 }
 
 // One workgroup per (row, KV head); thread = key.  The sum of one token's heads is added to the total as one number, so
@@ -145,11 +155,11 @@ extern "C" int psi_hip_kv_observe_weights(psi_hip_ctx* ctx, const psi_hip_gqa_co
         PSI_HIP_CHECK(hipGetLastError());
         return PSI_HIP_OK;
     }
-    const dim3 stats_grid(num_rows * g.hq), sum_grid(num_rows * g.hkv), join_grid((max_window * g.hq + 255) / 256, num_windows);
+    const dim3 stats_grid(num_rows * g.hq), sum_grid(num_rows * g.hkv);
 #define PSI_OBSERVE(TAG)                                                                                   \
     do {                                                                                                   \
         hipLaunchKernelGGL(observe_stats_generic<TAG>, stats_grid, dim3(64), 0, ctx->stream, a);           \
-        hipLaunchKernelGGL(observe_join, join_grid, dim3(256), 0, ctx->stream, a);                         \
+        launch_observe_join(ctx, a);                                                                       \
         hipLaunchKernelGGL(observe_sum_generic<TAG>, sum_grid, dim3(256), 0, ctx->stream, a);              \
     } while (0)
     if (g.dtype == PSI_HIP_F32) PSI_OBSERVE(F32Tag);

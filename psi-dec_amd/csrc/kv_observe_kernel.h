@@ -1,24 +1,30 @@
 // gfx950 observation kernels for 2-byte K and head_dim 128 or 256, any page size.
 //
-// One workgroup (8 waves) = one (row of keys, KV head).  The window's columns are staged in LDS in the operand order of
-// the matrix product, up to 256 at a time; a wave takes 64 keys at a time straight from their pages into registers, in
-// the operand order too (as in split_kv_decode_kernel.h: lane = token lane%16, 8-dim chunk lane/16, a 128-bit load per
-// 32 dims), and multiplies them with one block of 16 columns after the other.  Waves share nothing but the columns, so
-// there is no barrier in the loop over keys.  64 keys to a wave: a column operand read from LDS (8 cycles of the
-// compute unit's LDS) then feeds four products (64 cycles of a SIMD), which the four SIMDs' reads just fill half of.
+// One workgroup = one (row of keys, KV head).  The window's columns are staged in LDS in the operand order of the matrix
+// product; a wave takes 16 * kTiles keys at a time straight from their pages into registers, in the operand order too (as
+// in split_kv_decode_kernel.h: lane = token lane%16, 8-dim chunk lane/16, a 128-bit load per 32 dims), and multiplies
+// them with one block of 16 columns after the other.  The keys stay in registers for all columns, so that a column
+// operand read from LDS (8 cycles of the compute unit's LDS) feeds kTiles products (16 cycles of a SIMD each), and waves
+// share nothing but the columns: there is no barrier in the loops over keys and columns.
 //
-// A result lane holds 16 keys of one column, so the maximum and sum of a column (first pass) stay in the lane until the
-// row's end, and the weights of a key (second pass) are summed over the columns of a lane first and over the lanes once
-// per 64 keys.
+// A result lane holds 4 * kTiles keys of one column: the maximum and sum of a column (first pass) are reduced over the
+// lane and then over the four lanes of the column, the weights of a key (second pass) over the columns of a lane first
+// and over the lanes once per turn.
+//
+// Measured: 8 prompts of 1k-8k (bf16, D 256, 32 tokens, 24 heads over 4) 66 us for two walks of 73 MB and 2 * 14 GFLOP;
+// one prompt of 65536 (D 128, 64 tokens, 40 heads over 8) 127 us for 2 * 134 MB and 2 * 43 GFLOP, 670 TFLOP/s.  The first
+// is bound by what a workgroup does once (columns to LDS, first lines, joins: half of its time remains with a single
+// step of columns), the second by the matrix products and the exponentials, which share a SIMD's issue.
 #pragma once
 #include "kv_observe.h"
 #include "split_kv_decode_kernel.h"
 
 namespace psi {
 
-constexpr int kObserveWaves = 8, kObserveThreads = 64 * kObserveWaves;
-constexpr int kObserveTiles = 4;                      // 16-key tiles of a wave's turn
-constexpr uint32_t kObserveKeys = 16 * kObserveTiles;
+// Normalisers are joined inside the second pass as long as (rows of a window) * (columns) stays within this: at 160 and
+// 1460 that saves the 2 us of a launch (13.3 for 15.1 us, 65.9 for 67.6 us in all); at 10240 the two come out even, and
+// beyond, every workgroup would repeat a join that grows with the row count.
+constexpr uint64_t kFusedJoins = 8192;
 
 template <int kCtrl>
 __device__ __forceinline__ float dpp_of(float x) {
@@ -44,15 +50,25 @@ __device__ __forceinline__ float row_sums(float (&v)[16], uint32_t lane) {
     return v[0];
 }
 
+// Barrier that orders LDS only: K lines that a wave has asked for stay on their way.
+__device__ __forceinline__ void lds_barrier() {
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+}
+
 // kSum false: the maxima and sums of the row's columns.  kSum true: the weights.
-template <typename Tag, int D, int kMaxBlocks, bool kSum>
-__global__ __launch_bounds__(kObserveThreads, 2) void observe_kernel(ObserveArgs a) {
+template <typename Tag, int D, int kTiles, int kBlocks, int kMaxBlocks, int kWaves, bool kSum>
+__global__ __launch_bounds__(64 * kWaves, kWaves / 4) void observe_kernel(ObserveArgs a) {
+    static_assert(kMaxBlocks % kBlocks == 0, "whole steps of columns");
     constexpr int kSteps = D / 32;
-    constexpr uint32_t kColumns = 16 * kMaxBlocks, kChunks = D / 8;
+    constexpr uint32_t kThreads = 64 * kWaves, kColumns = 16 * kMaxBlocks, kChunks = D / 8;
+    constexpr int kWords = (kTiles + 3) / 4;
+    constexpr uint32_t kKeys = 16 * kTiles, kTurn = kWaves * kKeys;  // keys of a wave's turn, of all waves'
     __shared__ __attribute__((aligned(16))) uint4 q_lds[kMaxBlocks * kSteps * 64];
-    __shared__ int last_lds[kColumns];                        // last key that a column sees
+    __shared__ int last_lds[kColumns];                                  // last key of the row that a column sees
     __shared__ float lse_lds[kSum ? kColumns : 1];
-    __shared__ float2 merge_lds[kSum ? 1 : kObserveWaves][kSum ? 1 : kColumns];
+    __shared__ float2 state_lds[kSum ? 1 : kWaves][kSum ? 1 : kColumns];  // maximum and sum so far
 
     const uint32_t row = blockIdx.x / a.v.hkv, kv_head = blockIdx.x % a.v.hkv;
     const uint32_t tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -65,169 +81,220 @@ __global__ __launch_bounds__(kObserveThreads, 2) void observe_kernel(ObserveArgs
     const uint32_t columns = r.num_q * a.group;
 
     for (uint32_t c0 = 0; c0 < columns; c0 += kColumns) {
-        const uint32_t count = min(columns - c0, kColumns), blocks = (count + 15) / 16;
+        const uint32_t count = min(columns - c0, kColumns), blocks = (count + 16 * kBlocks - 1) / (16 * kBlocks) * kBlocks;
         const uint32_t key_end = min(r.end, r.position + (c0 + count - 1) / a.group + 1);  // what the last column sees
-        if (c0 > 0) __syncthreads();
-        for (uint32_t i = tid; i < blocks * 16 * kChunks; i += kObserveThreads) {
-            const uint32_t column = i / kChunks, chunk = i % kChunks, c = c0 + column;
-            uint4 value = make_uint4(0, 0, 0, 0);
-            if (c < columns)
-                value = *reinterpret_cast<const uint4*>(
-                    q + ((uint64_t)(r.q_begin + c / a.group) * a.hq + kv_head * a.group + c % a.group) * D + chunk * 8);
-            q_lds[((column / 16) * kSteps + chunk / 4) * 64 + (chunk % 4) * 16 + column % 16] = value;
-        }
-        for (uint32_t i = tid; i < blocks * 16; i += kObserveThreads) {
-            const uint32_t c = c0 + i;
-            last_lds[i] = c < columns ? (int)(r.position + c / a.group) : -1;
-            if constexpr (kSum) lse_lds[i] = c < columns ? join_column(a, r, kv_head, c) : INFINITY;
-        }
-        __syncthreads();
-
-        float col_max[kSum ? 1 : kMaxBlocks], col_sum[kSum ? 1 : kMaxBlocks];
-        if constexpr (!kSum) {
+        // The page IDs of a wave's turn are asked for a turn ahead.  Its lines are not: a second buffer of them costs the
+        // registers of a wave in three, and the other waves of the SIMD fill the wait better (one prompt of 65536, 64
+        // tokens: 78 and 60 us a pass with two buffers, 68 and 57 with one).
+        uint32_t next_ids[kTiles];
+        auto fetch_ids = [&](uint32_t base) __attribute__((always_inline)) {
 #pragma unroll
-            for (int b = 0; b < kMaxBlocks; ++b) {
-                col_max[b] = kEmptyMax;
-                col_sum[b] = 0.0f;
-            }
-        }
-        // page IDs of the wave's next 64 keys, a turn ahead of their lines
-        uint32_t page_id[kObserveTiles];
-        auto fetch_ids = [&](uint32_t base) {
-#pragma unroll
-            for (int t = 0; t < kObserveTiles; ++t) {
-                const uint32_t p = min(base + t * 16 + lane_row, key_end - 1);
-                page_id[t] = page_of(a.v, table, p, a.v.num_pages);
-            }
+            for (int t = 0; t < kTiles; ++t)
+                next_ids[t] = page_of(a.v, table, min(base + t * 16 + lane_row, key_end - 1), a.v.num_pages);
         };
-        uint32_t base = r.begin + wave * kObserveKeys;
-        if (base < key_end) fetch_ids(base);
-        for (; base < key_end; base += kObserveWaves * kObserveKeys) {
-            uint4 k[kObserveTiles][kSteps];
+        struct Keys {
+            uint4 line[kTiles][kSteps];
+            uint64_t missing[kWords];  // keys on pages beyond the arena: bit t % 4 * 16 + row of word t / 4
+        };
+        auto fetch_lines = [&](uint32_t base, Keys& k) __attribute__((always_inline)) {
             bool bad = false;
 #pragma unroll
-            for (int t = 0; t < kObserveTiles; ++t) {
+            for (int t = 0; t < kTiles; ++t) {
                 const uint32_t p = min(base + t * 16 + lane_row, key_end - 1);
-                const bool missing = page_id[t] == kNoPage;
+                const bool missing = next_ids[t] == kNoPage;
                 bad |= missing;
-                const uint16_t* line = pages + line_index(a.v, missing ? 0 : page_id[t], 0, kv_head, page_place(a.v, p)) +
+                const uint16_t* line = pages + line_index(a.v, missing ? 0 : next_ids[t], 0, kv_head, page_place(a.v, p)) +
                                        lane_quarter * 8;
 #pragma unroll
-                for (int i = 0; i < kSteps; ++i) k[t][i] = stream_load_b128(line + i * 32);
+                for (int i = 0; i < kSteps; ++i) k.line[t][i] = stream_load_b128(line + i * 32);
             }
-            // keys on pages beyond the arena: bit t * 16 + row, the same for the four quarters
-            uint64_t missing_keys = 0;
+#pragma unroll
+            for (int w = 0; w < kWords; ++w) k.missing[w] = 0;
             if (__any(bad)) {
                 report_cache_range(a.status);
 #pragma unroll
-                for (int t = 0; t < kObserveTiles; ++t)
-                    missing_keys |= (__ballot(page_id[t] == kNoPage) & 0xffffull) << (16 * t);
+                for (int t = 0; t < kTiles; ++t)
+                    k.missing[t / 4] |= (__ballot(next_ids[t] == kNoPage) & 0xffffull) << (16 * (t % 4));
             }
-            if (base + kObserveWaves * kObserveKeys < key_end) fetch_ids(base + kObserveWaves * kObserveKeys);
-            const bool masked = base + kObserveKeys > r.position + 1 || missing_keys != 0;
+        };
+        Keys k;
+        uint32_t base = r.begin + wave * kKeys;
+        if (base < key_end) {
+            fetch_ids(base);
+            fetch_lines(base, k);  // on their way while the columns are staged
+            if (base + kTurn < key_end) fetch_ids(base + kTurn);
+        }
 
-            auto logits_of = [&](uint32_t block, f32x4_t (&acc)[kObserveTiles]) __attribute__((always_inline)) {
+        if (c0 > 0) __syncthreads();
+        constexpr int kStage = 4;  // units of a thread under way
+        const uint32_t units = blocks * 16 * kChunks;
+        for (uint32_t i0 = tid; i0 < units; i0 += kThreads * kStage) {
+            uint4 value[kStage];
 #pragma unroll
-                for (int t = 0; t < kObserveTiles; ++t) acc[t] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
+            for (int u = 0; u < kStage; ++u) {
+                const uint32_t i = i0 + u * kThreads, c = c0 + i / kChunks;
+                const bool there = i < units && c < columns;
+                const uint64_t q_row = (uint64_t)(r.q_begin + c / a.group) * a.hq + kv_head * a.group + c % a.group;
+                value[u] = *reinterpret_cast<const uint4*>(q + (there ? q_row * D + i % kChunks * 8 : 0));
+                if (!there) value[u] = make_uint4(0, 0, 0, 0);
+            }
 #pragma unroll
-                for (int i = 0; i < kSteps; ++i) {
-                    const uint4 qv = q_lds[(block * kSteps + i) * 64 + lane];
+            for (int u = 0; u < kStage; ++u) {
+                const uint32_t i = i0 + u * kThreads, column = i / kChunks, chunk = i % kChunks;
+                if (i < units)
+                    q_lds[((column / 16) * kSteps + chunk / 4) * 64 + (chunk % 4) * 16 + column % 16] = value[u];
+            }
+        }
+        for (uint32_t i = tid; i < blocks * 16; i += kThreads) {
+            const uint32_t c = c0 + i;
+            last_lds[i] = c < columns ? (int)min(r.position + c / a.group, key_end - 1) : -1;
+            if constexpr (kSum)
+                lse_lds[i] = c >= columns ? INFINITY
+                             : a.lse != nullptr
+                                 ? a.lse[(uint64_t)(r.q_begin + c / a.group) * a.hq + kv_head * a.group + c % a.group]
+                                 : join_column(a, r, kv_head, c);
+        }
+        if constexpr (!kSum)
+            for (uint32_t i = lane; i < blocks * 16; i += 64) state_lds[wave][i] = make_float2(kEmptyMax, 0.0f);
+        lds_barrier();
+
+        for (; base < key_end; base += kTurn) {
+            bool masked = base + kKeys > min(r.position + 1, key_end);
 #pragma unroll
-                    for (int t = 0; t < kObserveTiles; ++t) acc[t] = mfma_16x16x32<Tag>(k[t][i], qv, acc[t]);
+            for (int w = 0; w < kWords; ++w) masked |= k.missing[w] != 0;
+            float sums[kWords][16];
+            if constexpr (kSum) {
+#pragma unroll
+                for (int w = 0; w < kWords; ++w)
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) sums[w][i] = 0.0f;
+            }
+            for (uint32_t b0 = 0; b0 < blocks; b0 += kBlocks) {
+                // kBlocks blocks at a time: independent products and exponentials to fill each other's latencies
+                f32x4_t acc[kBlocks][kTiles];
+#pragma unroll
+                for (int h = 0; h < kBlocks; ++h) {
+#pragma unroll
+                    for (int t = 0; t < kTiles; ++t) acc[h][t] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                    for (int i = 0; i < kSteps; ++i) {
+                        const uint4 qv = q_lds[((b0 + h) * kSteps + i) * 64 + lane];
+#pragma unroll
+                        for (int t = 0; t < kTiles; ++t) acc[h][t] = mfma_16x16x32<Tag>(k.line[t][i], qv, acc[h][t]);
+                    }
                 }
                 if (masked) {
-                    const int last = last_lds[block * 16 + lane_row];
 #pragma unroll
-                    for (int t = 0; t < kObserveTiles; ++t)
+                    for (int h = 0; h < kBlocks; ++h) {
+                        const int last = last_lds[(b0 + h) * 16 + lane_row];
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            const uint32_t at = t * 16 + lane_quarter * 4 + e;
-                            if ((int)(base + at) > last || (missing_keys >> at & 1)) acc[t][e] = -INFINITY;
-                        }
+                        for (int t = 0; t < kTiles; ++t)
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) {
+                                const uint32_t at = lane_quarter * 4 + e;
+                                if ((int)(base + t * 16 + at) > last || (k.missing[t / 4] >> (t % 4 * 16 + at) & 1))
+                                    acc[h][t][e] = -INFINITY;
+                            }
+                    }
                 }
-            };
-            if constexpr (!kSum) {
 #pragma unroll
-                for (int b = 0; b < kMaxBlocks; ++b) {
-                    if (b >= (int)blocks) continue;
-                    f32x4_t acc[kObserveTiles];
-                    logits_of(b, acc);
-                    float top = acc[0][0];
+                for (int h = 0; h < kBlocks; ++h) {
+                    const uint32_t column = (b0 + h) * 16 + lane_row;
+                    if constexpr (!kSum) {
+                        const float2 old = state_lds[wave][column];
+                        float top = acc[h][0][0];
 #pragma unroll
-                    for (int t = 0; t < kObserveTiles; ++t)
+                        for (int t = 0; t < kTiles; ++t)
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) top = fmaxf(top, acc[t][e]);
-                    const float next = fmaxf(col_max[b], top * a.scale_log2);
-                    float sum = 0.0f;
+                            for (int e = 0; e < 4; ++e) top = fmaxf(top, acc[h][t][e]);
+                        const float next = fmaxf(old.x, quarter_wave_max(top) * a.scale_log2);
+                        float sum = 0.0f;
 #pragma unroll
-                    for (int t = 0; t < kObserveTiles; ++t)
+                        for (int t = 0; t < kTiles; ++t)
 #pragma unroll
-                        for (int e = 0; e < 4; ++e)
-                            sum += __builtin_amdgcn_exp2f(fmaf(acc[t][e], a.scale_log2, -next));
-                    col_sum[b] = fmaf(col_sum[b], __builtin_amdgcn_exp2f(col_max[b] - next), sum);
-                    col_max[b] = next;
+                            for (int e = 0; e < 4; ++e)
+                                sum += __builtin_amdgcn_exp2f(fmaf(acc[h][t][e], a.scale_log2, -next));
+                        sum = fmaf(old.y, __builtin_amdgcn_exp2f(old.x - next), quarter_wave_sum(sum));
+                        if (lane < 16) state_lds[wave][column] = make_float2(next, sum);
+                    } else {
+                        const float lse = lse_lds[column];
+#pragma unroll
+                        for (int t = 0; t < kTiles; ++t)
+#pragma unroll
+                            for (int e = 0; e < 4; ++e)
+                                sums[t / 4][t % 4 * 4 + e] += __builtin_amdgcn_exp2f(fmaf(acc[h][t][e], a.scale_log2, -lse));
+                    }
                 }
-            } else {
-                float sums[16];
+            }
+            if constexpr (kSum) {
+                // lane_row's value of a word: of tile lane_row / 4, key lane_quarter * 4 + lane_row % 4 of it
 #pragma unroll
-                for (int i = 0; i < 16; ++i) sums[i] = 0.0f;
-                for (uint32_t b = 0; b < blocks; ++b) {
-                    f32x4_t acc[kObserveTiles];
-                    logits_of(b, acc);
-                    const float lse = lse_lds[b * 16 + lane_row];
-#pragma unroll
-                    for (int t = 0; t < kObserveTiles; ++t)
-#pragma unroll
-                        for (int e = 0; e < 4; ++e)
-                            sums[t * 4 + e] += __builtin_amdgcn_exp2f(fmaf(acc[t][e], a.scale_log2, -lse));
+                for (int w = 0; w < kWords; ++w) {
+                    const float sum = row_sums(sums[w], lane);
+                    const uint32_t tile = lane_row / 4, at = tile * 16 + lane_quarter * 4 + lane_row % 4, p = base + w * 64 + at;
+                    if (w * 4 + tile < kTiles && p < key_end && !(k.missing[w] >> at & 1))
+                        add_weight(a, r, table, kv_head, p, sum, c0 == 0);
                 }
-                const float sum = row_sums(sums, lane);  // of tile lane_row / 4, token lane_quarter * 4 + lane_row % 4
-                const uint32_t at = lane_row / 4 * 16 + lane_quarter * 4 + lane_row % 4, p = base + at;
-                if (p < key_end && !(missing_keys >> at & 1)) add_weight(a, r, table, kv_head, p, sum, c0 == 0);
+            }
+            if (base + kTurn < key_end) {
+                fetch_lines(base + kTurn, k);
+                if (base + 2 * kTurn < key_end) fetch_ids(base + 2 * kTurn);
             }
         }
         if constexpr (!kSum) {
-#pragma unroll
-            for (int b = 0; b < kMaxBlocks; ++b) {
-                if (b >= (int)blocks) continue;
-                const float m = quarter_wave_max(col_max[b]);
-                const float s = quarter_wave_sum(col_sum[b] * __builtin_amdgcn_exp2f(col_max[b] - m));
-                if (lane < 16) merge_lds[wave][b * 16 + lane] = make_float2(m, s);
-            }
-            __syncthreads();
-            for (uint32_t i = tid; i < count; i += kObserveThreads) {
+            lds_barrier();
+            for (uint32_t i = tid; i < count; i += kThreads) {
                 float m = kEmptyMax, s = 0.0f;
 #pragma unroll
-                for (int w = 0; w < kObserveWaves; ++w) m = fmaxf(m, merge_lds[w][i].x);
+                for (int w = 0; w < kWaves; ++w) m = fmaxf(m, state_lds[w][i].x);
 #pragma unroll
-                for (int w = 0; w < kObserveWaves; ++w)
-                    s = fmaf(merge_lds[w][i].y, __builtin_amdgcn_exp2f(merge_lds[w][i].x - m), s);
+                for (int w = 0; w < kWaves; ++w) {
+                    const float2 part = state_lds[w][i];
+                    s = fmaf(part.y, __builtin_amdgcn_exp2f(part.x - m), s);
+                }
                 a.stats[stat_index(a, row, kv_head, c0 + i)] = make_float2(m, s);
             }
         } else {
             // positions of the row that no column of the first columns sees still get their turn's base
             if (c0 == 0)
-                for (uint32_t p = max(key_end, r.begin) + tid; p < r.end; p += kObserveThreads)
+                for (uint32_t p = max(key_end, r.begin) + tid; p < r.end; p += kThreads)
                     if (page_of(a.v, table, p, a.v.num_pages) != kNoPage) add_weight(a, r, table, kv_head, p, 0.0f, true);
         }
     }
 }
 
-template <typename Tag, int D, int kMaxBlocks>
+// kTiles, kBlocks, kWaves of either pass.  Three waves a SIMD of 160 registers each: with two (and twice the keys or
+// columns in flight) the batch of eight prompts, 32 tokens each, takes 36 + 34 us for 32 + 31, with four the lines spill.
+template <int kTiles_, int kBlocks_, int kWaves_>
+struct ObservePass {
+    static constexpr int kTiles = kTiles_, kBlocks = kBlocks_, kWaves = kWaves_;
+};
+template <typename Tag, int D, int kMaxBlocks, typename Stats, typename Sum>
 inline void launch_observe_blocks(psi_hip_ctx* ctx, const ObserveArgs& a) {
-    const dim3 grid(a.num_rows * a.v.hkv), threads(kObserveThreads);
-    hipLaunchKernelGGL((observe_kernel<Tag, D, kMaxBlocks, false>), grid, threads, 0, ctx->stream, a);
-    hipLaunchKernelGGL((observe_kernel<Tag, D, kMaxBlocks, true>), grid, threads, 0, ctx->stream, a);
+    const dim3 grid(a.num_rows * a.v.hkv);
+    ObserveArgs fused = a;
+    const uint64_t joins = (uint64_t)a.num_rows / a.num_windows * a.max_window * a.group;
+    if (joins <= kFusedJoins) fused.lse = nullptr;
+    hipLaunchKernelGGL((observe_kernel<Tag, D, Stats::kTiles, Stats::kBlocks, kMaxBlocks, Stats::kWaves, false>), grid,
+                       dim3(64 * Stats::kWaves), 0, ctx->stream, a);
+    if (fused.lse != nullptr) launch_observe_join(ctx, a);
+    hipLaunchKernelGGL((observe_kernel<Tag, D, Sum::kTiles, Sum::kBlocks, kMaxBlocks, Sum::kWaves, true>), grid,
+                       dim3(64 * Sum::kWaves), 0, ctx->stream, fused);
 }
 template <typename Tag>
 inline void launch_observe(psi_hip_ctx* ctx, const ObserveArgs& a) {
+    // few columns: a fraction of the LDS, which launches faster (8 tokens over a prompt of 777: 13.3 for 14.2 us)
     const bool narrow = (uint64_t)a.max_window * a.group <= 64;
     if (a.v.d == 256) {
-        if (narrow) launch_observe_blocks<Tag, 256, 4>(ctx, a);
-        else launch_observe_blocks<Tag, 256, 16>(ctx, a);
+        using Pass = ObservePass<2, 2, 12>;
+        if (narrow) launch_observe_blocks<Tag, 256, 4, Pass, Pass>(ctx, a);
+        else launch_observe_blocks<Tag, 256, 16, Pass, Pass>(ctx, a);
     } else {
-        if (narrow) launch_observe_blocks<Tag, 128, 4>(ctx, a);
-        else launch_observe_blocks<Tag, 128, 16>(ctx, a);
+        // 64 keys a turn for the maxima (68 us; 78 with 32), 32 for the weights, whose sums need registers too (57; 58 with 48)
+        using Stats = ObservePass<4, 1, 12>;
+        using Sum = ObservePass<2, 2, 12>;
+        if (narrow) launch_observe_blocks<Tag, 128, 4, Sum, Sum>(ctx, a);
+        else launch_observe_blocks<Tag, 128, 24, Stats, Sum>(ctx, a);
     }
 }
 
