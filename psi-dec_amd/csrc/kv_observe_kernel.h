@@ -11,10 +11,10 @@
 // lane and then over the four lanes of the column, the weights of a key (second pass) over the columns of a lane first
 // and over the lanes once per turn.
 //
-// Measured: 8 prompts of 1k-8k (bf16, D 256, 32 tokens, 24 heads over 4) 66 us for two walks of 73 MB and 2 * 14 GFLOP;
-// one prompt of 65536 (D 128, 64 tokens, 40 heads over 8) 127 us for 2 * 134 MB and 2 * 43 GFLOP, 670 TFLOP/s.  The first
-// is bound by what a workgroup does once (columns to LDS, first lines, joins: half of its time remains with a single
-// step of columns), the second by the matrix products and the exponentials, which share a SIMD's issue.
+// Measured: 8 prompts of 1k-8k (bf16, D 256, 32 tokens, 24 heads over 4) 58 us for two walks of 75 MB and 2 * 14 GFLOP;
+// one prompt of 65536 (D 128, 64 tokens, 40 heads over 8) 119 us for 2 * 134 MB and 2 * 43 GFLOP, 720 TFLOP/s.  The first
+// is bound by the lines: a workgroup has two turns, each a burst of reads and then a wait (27 of 33 us of its first pass
+// remained with a sixth of the products).  The second is bound by products and exponentials, which share a SIMD's issue.
 #pragma once
 #include "kv_observe.h"
 #include "split_kv_decode_kernel.h"
@@ -22,7 +22,7 @@
 namespace psi {
 
 // Normalisers are joined inside the second pass as long as (rows of a window) * (columns) stays within this: at 160 and
-// 1460 that saves the 2 us of a launch (13.3 for 15.1 us, 65.9 for 67.6 us in all); at 10240 the two come out even, and
+// 1460 that saves the 2 us of a launch (13 for 15 us and 66 for 68 us in all); at 10240 the two come out even, and
 // beyond, every workgroup would repeat a join that grows with the row count.
 constexpr uint64_t kFusedJoins = 8192;
 
@@ -106,7 +106,7 @@ __global__ __launch_bounds__(64 * kWaves, kWaves / 4) void observe_kernel(Observ
                 const uint16_t* line = pages + line_index(a.v, missing ? 0 : next_ids[t], 0, kv_head, page_place(a.v, p)) +
                                        lane_quarter * 8;
 #pragma unroll
-                for (int i = 0; i < kSteps; ++i) k.line[t][i] = stream_load_b128(line + i * 32);
+                for (int i = 0; i < kSteps; ++i) k.line[t][i] = *reinterpret_cast<const uint4*>(line + i * 32);
             }
 #pragma unroll
             for (int w = 0; w < kWords; ++w) k.missing[w] = 0;
@@ -118,11 +118,17 @@ __global__ __launch_bounds__(64 * kWaves, kWaves / 4) void observe_kernel(Observ
             }
         };
         Keys k;
-        uint32_t base = r.begin + wave * kKeys;
-        if (base < key_end) {
+        // The second pass walks the turns backwards: what the first pass read last may still be in the cache of the XCD
+        // (27.3 for 28.8 us at 8 prompts of 1k-8k, the same at 65536).  Loads are ordinary ones for that reason: streaming
+        // ones take 33 + 31 us for 30 + 27, and 67 + 58 for 62 + 52 at 65536.
+        const uint32_t first = r.begin + wave * kKeys;
+        uint32_t turns = first < key_end ? (key_end - first + kTurn - 1) / kTurn : 0;
+        const uint32_t step = kSum ? 0 - kTurn : kTurn;
+        uint32_t base = kSum ? first + (turns - 1) * kTurn : first;
+        if (turns > 0) {
             fetch_ids(base);
             fetch_lines(base, k);  // on their way while the columns are staged
-            if (base + kTurn < key_end) fetch_ids(base + kTurn);
+            if (turns > 1) fetch_ids(base + step);
         }
 
         if (c0 > 0) __syncthreads();
@@ -158,7 +164,7 @@ __global__ __launch_bounds__(64 * kWaves, kWaves / 4) void observe_kernel(Observ
             for (uint32_t i = lane; i < blocks * 16; i += 64) state_lds[wave][i] = make_float2(kEmptyMax, 0.0f);
         lds_barrier();
 
-        for (; base < key_end; base += kTurn) {
+        for (; turns > 0; --turns, base += step) {
             bool masked = base + kKeys > min(r.position + 1, key_end);
 #pragma unroll
             for (int w = 0; w < kWords; ++w) masked |= k.missing[w] != 0;
@@ -236,9 +242,9 @@ __global__ __launch_bounds__(64 * kWaves, kWaves / 4) void observe_kernel(Observ
                         add_weight(a, r, table, kv_head, p, sum, c0 == 0);
                 }
             }
-            if (base + kTurn < key_end) {
-                fetch_lines(base + kTurn, k);
-                if (base + 2 * kTurn < key_end) fetch_ids(base + 2 * kTurn);
+            if (turns > 1) {
+                fetch_lines(base + step, k);
+                if (turns > 2) fetch_ids(base + 2 * step);
             }
         }
         if constexpr (!kSum) {
@@ -264,7 +270,7 @@ __global__ __launch_bounds__(64 * kWaves, kWaves / 4) void observe_kernel(Observ
 }
 
 // kTiles, kBlocks, kWaves of either pass.  Three waves a SIMD of 160 registers each: with two (and twice the keys or
-// columns in flight) the batch of eight prompts, 32 tokens each, takes 36 + 34 us for 32 + 31, with four the lines spill.
+// columns in flight) the batch of eight prompts, 32 tokens each, takes 36 + 31 us for 30 + 27, with four the lines spill.
 template <int kTiles_, int kBlocks_, int kWaves_>
 struct ObservePass {
     static constexpr int kTiles = kTiles_, kBlocks = kBlocks_, kWaves = kWaves_;
@@ -290,7 +296,7 @@ inline void launch_observe(psi_hip_ctx* ctx, const ObserveArgs& a) {
         if (narrow) launch_observe_blocks<Tag, 256, 4, Pass, Pass>(ctx, a);
         else launch_observe_blocks<Tag, 256, 16, Pass, Pass>(ctx, a);
     } else {
-        // 64 keys a turn for the maxima (68 us; 78 with 32), 32 for the weights, whose sums need registers too (57; 58 with 48)
+        // 64 keys a turn for the maxima (68 us with streaming loads, 78 with 32), 32 for the weights, whose sums need registers too (52; 53 with 48)
         using Stats = ObservePass<4, 1, 12>;
         using Sum = ObservePass<2, 2, 12>;
         if (narrow) launch_observe_blocks<Tag, 128, 4, Sum, Sum>(ctx, a);
