@@ -853,6 +853,12 @@ int psi_hip_split_kv_single_q_attend_weights(
     const psi_hip_kv_weights* weights, uint32_t gqa_layer_index, uint32_t num_total_tokens,
     uint32_t num_total_kv_splits, uint32_t num_active_tokens, uint32_t num_active_kv_splits);
 
+/* psi_hip_gqa_layer_record of a SingleQ batch whose attention accumulates these weights (TiledQ batches are refused: plan
+ * the batch with the SingleQ variant).  The layer's rotary positions are cache positions: see above for requests that
+ * were compacted. */
+int psi_hip_gqa_layer_record_weights(psi_hip_ctx* ctx, const psi_hip_gqa_layer_config* cfg,
+                                     const psi_hip_gqa_layer_input* input, const psi_hip_kv_weights* weights);
+
 /* Host plan of an observation: request r brings query tokens cu_tokens[r] .. cu_tokens[r + 1] (at least one) at positions
  * token_indices[r] ..; its keys are the cached positions up to each token's own.  num_held[r]: the positions whose
  * accumulators count already, the others start from zero (null: token_indices, as in a decode step; 0 for a prompt's

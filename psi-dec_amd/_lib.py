@@ -393,6 +393,8 @@ PROTOTYPES = {
         c_int, [c_void_p, _CFG, _LAYOUT, c_void_p, c_void_p, c_uint64, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
                 c_void_p, c_void_p, c_void_p, c_uint32, c_void_p, c_void_p, c_uint64, c_void_p,
                 POINTER(OutputGateStruct), POINTER(KVWeightsStruct), c_uint32, c_uint32, c_uint32, c_uint32, c_uint32]),
+    "psi_hip_gqa_layer_record_weights": (
+        c_int, [c_void_p, POINTER(LayerConfigStruct), POINTER(LayerInputStruct), POINTER(KVWeightsStruct)]),
     "psi_hip_kv_observe_plan": (
         c_int, [_CFG, _LAYOUT, _U32P, _U32P, _U32P, _U32P, c_uint32, _U32P, _U32P, c_uint32, _U32P, _U32P,
                 POINTER(c_uint64)]),

@@ -112,7 +112,9 @@ int check_input(const psi_hip_gqa_layer_input* in) {
     return PSI_HIP_OK;
 }
 
-int record_layer(psi_hip_ctx* ctx, const psi_hip_gqa_layer_config* cfg, const psi_hip_gqa_layer_input* in) {
+// With `weights`, the attention also accumulates the attention weights of the step (SingleQ batches).
+int record_layer(psi_hip_ctx* ctx, const psi_hip_gqa_layer_config* cfg, const psi_hip_gqa_layer_input* in,
+                 const psi_hip_kv_weights* weights = nullptr) {
     PSI_REQUIRE(ctx != nullptr, "ctx must not be null");
     LayerPlan plan;
     int rc = make_layer_plan(cfg, &plan);
@@ -126,6 +128,8 @@ int record_layer(psi_hip_ctx* ctx, const psi_hip_gqa_layer_config* cfg, const ps
     const psi_hip_page_table_layout* layout = &in->page_table_layout;
     const bool tiled = md.variant.kind == PSI_HIP_VARIANT_TILED_Q;
     const uint32_t layer = in->gqa_layer_index;
+    PSI_REQUIRE(!tiled || weights == nullptr,
+                "attention weights are accumulated by the SingleQ variant: prepare the batch with it");
 
     const void* q = in->q;
     psi_hip_output_gate gate_storage;
@@ -190,6 +194,13 @@ int record_layer(psi_hip_ctx* ctx, const psi_hip_gqa_layer_config* cfg, const ps
                                                s.num_total_q_token_tiles, s.num_total_kv_splits, s.num_q_token_tiles,
                                                md.partial_row_index, gate);
     }
+    if (weights != nullptr)
+        return psi_hip_split_kv_single_q_attend_weights(
+            ctx, acfg, layout, q, in->kv_pages, in->kv_pages_bytes, append_with_map ? in->k : nullptr,
+            append_with_map ? in->v : nullptr, md.req_slots, md.flat_token_indices, in->page_ids, md.kv_splits,
+            md.cu_kv_splits, md.worker_cu, md.worker_cu ? md.num_workers : 0, md.partial_row_index, in->partial_scratch,
+            in->partial_scratch_bytes, in->output, gate, weights, layer, s.num_total_tokens, s.num_total_kv_splits,
+            s.num_tokens, s.num_kv_splits);
     if (append_with_map)
         rc = psi_hip_kv_page_write_split_kv_single_q_map(
             ctx, acfg, layout, q, in->kv_pages, in->kv_pages_bytes, in->k, in->v, md.req_slots, md.flat_token_indices,
@@ -493,6 +504,12 @@ extern "C" int psi_hip_gqa_layer_advance_decode(const psi_hip_gqa_plan_options* 
 extern "C" int psi_hip_gqa_layer_record(psi_hip_ctx* ctx, const psi_hip_gqa_layer_config* cfg,
                                         const psi_hip_gqa_layer_input* input) {
     return record_layer(ctx, cfg, input);
+}
+
+extern "C" int psi_hip_gqa_layer_record_weights(psi_hip_ctx* ctx, const psi_hip_gqa_layer_config* cfg,
+                                                const psi_hip_gqa_layer_input* input, const psi_hip_kv_weights* weights) {
+    PSI_REQUIRE(weights != nullptr, "the accumulated weights must not be null");
+    return record_layer(ctx, cfg, input, weights);
 }
 
 extern "C" int psi_hip_gqa_layer_prepare_mixed(const psi_hip_gqa_layer_config* cfg,

@@ -269,8 +269,8 @@ __global__ __launch_bounds__(64 * kWaves, kWaves / 4) void observe_kernel(Observ
     }
 }
 
-// kTiles, kBlocks, kWaves of either pass.  Three waves a SIMD of 160 registers each: with two (and twice the keys or
-// columns in flight) the batch of eight prompts, 32 tokens each, takes 36 + 31 us for 30 + 27, with four the lines spill.
+// kTiles, kBlocks, kWaves of either pass.  Three waves a SIMD of 160 registers each: with two (and half again the
+// keys a turn) the batch of eight prompts, 32 tokens each, takes 36 + 31 us for 30 + 27, with four the lines spill.
 template <int kTiles_, int kBlocks_, int kWaves_>
 struct ObservePass {
     static constexpr int kTiles = kTiles_, kBlocks = kBlocks_, kWaves = kWaves_;
@@ -296,7 +296,8 @@ inline void launch_observe(psi_hip_ctx* ctx, const ObserveArgs& a) {
         if (narrow) launch_observe_blocks<Tag, 256, 4, Pass, Pass>(ctx, a);
         else launch_observe_blocks<Tag, 256, 16, Pass, Pass>(ctx, a);
     } else {
-        // 64 keys a turn for the maxima (68 us with streaming loads, 78 with 32), 32 for the weights, whose sums need registers too (52; 53 with 48)
+        // 64 keys a turn for the maxima (with streaming loads 68 us; 78 with 32), 32 for the weights, whose sums need
+        // registers too (57; 58 with 48)
         using Stats = ObservePass<4, 1, 12>;
         using Sum = ObservePass<2, 2, 12>;
         if (narrow) launch_observe_blocks<Tag, 128, 4, Sum, Sum>(ctx, a);

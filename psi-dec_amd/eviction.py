@@ -17,7 +17,8 @@ from typing import Optional, Sequence
 import numpy as np
 
 from . import _lib as L
-from .gqa import Device, Dtype, GQAPageTableLayout, _cfg_struct, _nbytes, _ptr, _tokens_per_page
+from .gqa import (Device, Dtype, GQAPageTableLayout, _cfg_struct, _check_page_weights, _nbytes, _ptr,
+                  _tokens_per_page)
 
 
 @dataclass(frozen=True)
@@ -57,13 +58,6 @@ def _u32(values):
 
 def _p(a):
     return a.ctypes.data_as(ctypes.POINTER(ctypes.c_uint32)) if a is not None else None
-
-
-def _check_weights(weights, device: Device):
-    import torch
-
-    if weights.dtype != torch.float32 or not weights.is_contiguous() or weights.device != device.torch_device:
-        raise ValueError("page_weights: a contiguous float32 tensor on the kernels' device is wanted")
 
 
 def _upload(device: Device, array: np.ndarray):
@@ -117,7 +111,7 @@ class GQAKVObserveKernels:
     def invoke(self, plan: GQAKVObservePlan, q, kv_pages, page_ids, page_weights, page_table_index: int,
                decay: float = 1.0):
         """Adds the windows' weights to `page_weights`; `q`: [query tokens][Q heads][head_dim], rotated."""
-        _check_weights(page_weights, self.device)
+        _check_page_weights(page_weights, self.device)
         if q.numel() < plan.num_q_tokens * self.config.num_q_heads * self.config.head_dim or not q.is_contiguous():
             raise ValueError("q: contiguous rows for every planned query token are wanted")
         L.check(self.device.lib.psi_hip_kv_observe_weights(
@@ -174,7 +168,7 @@ class GQAKVEvictionKernels:
     def invoke_select(self, plan: GQAKVEvictionPlan, page_weights, page_ids, page_table_index: int):
         """The positions to keep, int32 [requests][KV heads][budget], ascending and padded with -1 (the 32-bit
         sentinel); `plan.kept`, which the plan's next selection writes again."""
-        _check_weights(page_weights, self.device)
+        _check_page_weights(page_weights, self.device)
         L.check(self.device.lib.psi_hip_kv_select_kept(
             self.device.ctx, ctypes.byref(self._cfg), ctypes.byref(self._layout), _ptr(page_weights),
             _nbytes(page_weights), _ptr(page_ids), _ptr(plan.requests), plan.num_reqs, plan.max_cached, self.budget,
@@ -186,7 +180,7 @@ class GQAKVEvictionKernels:
         import torch
 
         if page_weights is not None:
-            _check_weights(page_weights, self.device)
+            _check_page_weights(page_weights, self.device)
         if kept.dtype != torch.int32 or not kept.is_contiguous() or kept.numel() != plan.kept.numel():
             raise ValueError("kept: the contiguous int32 [requests][KV heads][budget] of a selection is wanted")
         L.check(self.device.lib.psi_hip_kv_compact(

@@ -1027,6 +1027,27 @@ class GQASplitKVSingleQLogits:
             self.buffer = torch.empty(self.bytes, dtype=torch.uint8, device=device.torch_device)
 
 
+def _check_page_weights(weights, device: Device):
+    import torch
+
+    if weights.dtype != torch.float32 or not weights.is_contiguous() or weights.device != device.torch_device:
+        raise ValueError("page_weights: a contiguous float32 tensor on the kernels' device is wanted")
+
+
+@dataclass
+class GQAKVWeights:
+    """psi_hip_kv_weights: what a decode step adds its attention weights to (`page_weights` of eviction.py) and the
+    logits it goes through; tokens cached before the step keep `decay` times what they had."""
+    page_weights: object
+    logits: GQASplitKVSingleQLogits
+    decay: float = 1.0
+
+    def struct(self, device: Device):
+        _check_page_weights(self.page_weights, device)
+        return L.KVWeightsStruct(self.page_weights.data_ptr(), _nbytes(self.page_weights), self.logits.buffer.data_ptr(),
+                                 self.logits.bytes, self.logits.max_context_tokens, self.decay)
+
+
 class GQASplitKVSingleQKernels:
     def __init__(self, device: Device, config: GQASplitKVSingleQConfig, shape: GQASplitKVSingleQShape):
         config.num_tokens_per_page()
@@ -1104,8 +1125,7 @@ class GQASplitKVSingleQKernels:
         token's attention weight to `page_weights`, f32 [pages][KV heads][tokens per page] (see `eviction.py`):
         tokens cached before this step keep `decay` times what they had, this step's own start from zero."""
         cfg, layout = self.config.struct(), self.config.page_table_layout.struct()
-        weights = L.KVWeightsStruct(page_weights.data_ptr(), _nbytes(page_weights), logits.buffer.data_ptr(),
-                                    logits.bytes, logits.max_context_tokens, decay)
+        weights = GQAKVWeights(page_weights, logits, decay).struct(self.device)
         L.check(self.device.lib.psi_hip_split_kv_single_q_attend_weights(
             self.device.ctx, ctypes.byref(cfg), ctypes.byref(layout), _ptr(q), _ptr(kv_pages), _nbytes(kv_pages),
             _ptr(flat_k), _ptr(flat_v), _ptr(req_slots), _ptr(flat_token_indices), _ptr(page_ids),
@@ -1331,6 +1351,7 @@ class GQAInput:
     output: object = None
     shape: Optional[GQAReplayShape] = None  # overrides batch_metadata.replay_shape() (e.g. wider capacities)
     counts_uploaded: bool = False  # a replay cache reads the count words the metadata upload brought along
+    kv_weights: Optional[GQAKVWeights] = None  # `record` of a SingleQ batch accumulates its attention weights there
 
 
 @dataclass
@@ -1382,6 +1403,12 @@ class GQA:
 
     def new_scratch(self, max_tokens: int, max_kv_splits: Optional[int] = None) -> GQAScratch:
         return GQAScratch(self.device, self, max_tokens, max_kv_splits)
+
+    def new_logits(self, max_tokens: int, max_context_tokens: int) -> GQASplitKVSingleQLogits:
+        """Room for `GQAInput.kv_weights`: steps of up to `max_tokens` tokens whose contexts stay within
+        `max_context_tokens`."""
+        return GQASplitKVSingleQLogits(self.device, self.split_kv.config, GQASplitKVSingleQShape(max_tokens, 1),
+                                       max_context_tokens)
 
     def select_variant(self, batch_metadata, token_indices, cu_tokens, policy=None) -> GQASplitKVVariant:
         return select_split_kv_variant(self.split_kv, batch_metadata.max_tokens(), policy, token_indices, cu_tokens)
@@ -1464,8 +1491,10 @@ class GQA:
                                                                ctypes.byref(p)))
         return keep[1]
 
-    def input_struct(self, inp: GQAInput):
+    def input_struct(self, inp: GQAInput, takes_weights: bool = False):
         """(psi_hip_gqa_layer_input, keep-alive objects) for an input."""
+        if inp.kv_weights is not None and not takes_weights:
+            raise ValueError("kv_weights: only `record` accumulates attention weights")
         md = inp.batch_metadata.struct(inp.shape, counts_uploaded=inp.counts_uploaded)
         sc = inp.scratch
         qgkv = inp.qgkv if (inp.qgkv is not None or inp.q is not None) else sc.qgkv
@@ -1481,9 +1510,15 @@ class GQA:
 
     def record(self, inp: GQAInput):
         """`GQA::record` (backend.rs:394-658): issues the layer's launches on the device's stream and returns
-        the output buffer (the reference returns the caller-owned buffer it was given, too)."""
+        the output buffer (the reference returns the caller-owned buffer it was given, too).  With `inp.kv_weights`
+        the attention also accumulates its weights (psi_hip_gqa_layer_record_weights; not in the reference)."""
         cfg = self.struct()
-        s, keep = self.input_struct(inp)
+        s, keep = self.input_struct(inp, takes_weights=True)
+        if inp.kv_weights is not None:
+            weights = inp.kv_weights.struct(self.device)
+            L.check(self.device.lib.psi_hip_gqa_layer_record_weights(self.device.ctx, ctypes.byref(cfg), ctypes.byref(s),
+                                                                     ctypes.byref(weights)))
+            return keep[1]
         L.check(self.device.lib.psi_hip_gqa_layer_record(self.device.ctx, ctypes.byref(cfg), ctypes.byref(s)))
         return keep[1]
 
