@@ -904,8 +904,9 @@ int psi_hip_kv_select_kept(psi_hip_ctx* ctx, const psi_hip_gqa_config* cfg, cons
 
 /* Moves the K and V lines, and the accumulators unless page_weights is null, of position kept[i] to position i, in
  * place, for every request of more than `budget` tokens.  The kept positions of a (request, head) ascend, as the
- * selection writes them; an entry that lies outside the cached tokens or below its own index moves nothing.  Positions
- * from `budget` on keep their bytes.  Not while device-side counts are bound. */
+ * selection writes them (in another order, the lines at its front are some of its cached lines); an entry that lies
+ * outside the cached tokens or below its own index moves nothing.  Positions from `budget` on keep their bytes.  Up to
+ * five launches for few long requests, otherwise one.  Not while device-side counts are bound. */
 int psi_hip_kv_compact(psi_hip_ctx* ctx, const psi_hip_gqa_config* cfg, const psi_hip_page_table_layout* layout,
                        void* kv_pages, uint64_t kv_pages_bytes, float* page_weights, uint64_t page_weights_bytes,
                        const uint32_t* page_ids, const uint32_t* requests, uint32_t num_reqs,

@@ -5,6 +5,12 @@
 // is read whole before any of it is written.  What run j writes lies below the run's end, and every entry beyond that
 // end reads a position at or beyond it, so later runs still find their lines.  Runs of one line slice must follow one
 // another, but slices of a line (a few 16-byte chunks of K or of V) and heads are independent: a workgroup owns one.
+//
+// Few requests give few such workgroups, and a run waits for memory once.  Then most lines move in launches of their own
+// that need no order within: call an entry of level 0 if its position lies at or beyond the budget, so that no entry
+// overwrites it, and of level k + 1 if its position is that of an entry of level k, which overwrites it.  Entries of one
+// level read what lies outside the level, so a level moves at once, and higher levels have to move first.  As kept
+// ascends, higher levels are lower entries: the runs move what is left at the front, then the levels follow, 0 last.
 #include "kv_eviction.h"
 
 namespace psi {
@@ -21,7 +27,34 @@ struct CompactArgs {
     uint32_t max_cached, budget;
     uint32_t line_units, slice_units, num_slices;  // units of a line, of a slice; slices of a line
     uint32_t num_reqs, group_stride;               // group_stride: workgroups between two slices of a line
+    uint32_t levels;                               // entries of lower levels move in launches of their own
 };
+
+// The request of a workgroup; false: there is nothing to move.
+__device__ __forceinline__ bool load_request(const CompactArgs& a, uint32_t req, uint32_t* slot, uint32_t* n) {
+    *slot = a.requests[req * kRequestWords];
+    *n = min(min(a.requests[req * kRequestWords + 1], a.max_cached), a.v.positions);
+    if (*n <= a.budget) return false;  // everything is kept where it is
+    if (*slot >= a.v.num_slots) {
+        report_cache_range(a.status);
+        return false;
+    }
+    return true;
+}
+
+// First of `count` ascending values that is `bound` or more, by a wave: 64 probes a step.
+__device__ __forceinline__ uint32_t lower_bound(const uint32_t* values, uint32_t count, uint32_t bound) {
+    const uint32_t lane = threadIdx.x & 63;
+    uint32_t lo = 0, hi = count;  // values below lo are less than bound, hi's (if any) is not
+    while (lo < hi) {
+        const uint32_t step = (hi - lo + 63) / 64, at = lo + lane * step;
+        const uint64_t reached = __ballot(at >= hi || values[min(at, hi - 1)] >= bound);
+        const uint32_t first = reached != 0 ? (uint32_t)__builtin_ctzll(reached) : 64;
+        if (first < 64) hi = min(hi, lo + first * step);
+        if (first > 0) lo = min(hi, lo + (first - 1) * step + 1);
+    }
+    return lo;
+}
 
 // The runs of one (request, KV head, slice): a workgroup takes `per_step` lines at a time, a unit a lane, kUnroll
 // steps a run.  What a run's lines need is asked for ahead, a link of the chain per run: the kept positions two runs
@@ -29,8 +62,8 @@ struct CompactArgs {
 // the first unit of the array in place of a line, so that the loads of a run stand without branches between them.
 template <int kUnroll, typename Unit, typename Index>
 __device__ __forceinline__ void move_runs(const CompactArgs& a, const uint32_t* kept, const uint32_t* table, uint32_t n,
-                                          uint32_t num_pages, Unit* data, uint32_t my_line, uint32_t per_step, bool in_line,
-                                          Index index) {
+                                          uint32_t entries, uint32_t num_pages, Unit* data, uint32_t my_line,
+                                          uint32_t per_step, bool in_line, Index index) {
     const uint32_t per_run = per_step * kUnroll;
     uint32_t src[kUnroll], src_next[kUnroll], from[kUnroll], to[kUnroll];
     auto entry = [&](uint32_t base, int u) -> uint32_t { return base + u * per_step + my_line; };
@@ -38,7 +71,7 @@ __device__ __forceinline__ void move_runs(const CompactArgs& a, const uint32_t* 
 #pragma unroll
         for (int u = 0; u < kUnroll; ++u) {
             const uint32_t i = entry(base, u);
-            const bool there = in_line && i < a.budget;
+            const bool there = in_line && i < entries;
             const uint32_t k = kept[there ? i : 0];
             out[u] = there ? k : i;  // an entry that stays where it is moves nothing
         }
@@ -56,7 +89,7 @@ __device__ __forceinline__ void move_runs(const CompactArgs& a, const uint32_t* 
     fetch_kept(0, src);
     fetch_kept(per_run, src_next);
     fetch_pages(0, src);
-    for (uint32_t base = 0; base < a.budget; base += per_run) {
+    for (uint32_t base = 0; base < entries; base += per_run) {
         Unit held[kUnroll];
         uint64_t target[kUnroll];
         uint32_t moves = 0;
@@ -92,29 +125,100 @@ __global__ __launch_bounds__(kThreads) void compact_kernel(CompactArgs a) {
     const uint32_t pair = is_weights ? (blockIdx.x - line_groups) * 2 : blockIdx.x % a.group_stride;
     const uint32_t kind = pair % 2, kv_head = pair / 2 % a.v.hkv, req = pair / 2 / a.v.hkv;
     if (req >= a.num_reqs) return;
-    const uint32_t slot = a.requests[req * kRequestWords];
-    const uint32_t n = min(min(a.requests[req * kRequestWords + 1], a.max_cached), a.v.positions);
-    if (n <= a.budget) return;  // everything is kept where it is
-    if (slot >= a.v.num_slots) {
-        report_cache_range(a.status);
-        return;
-    }
+    uint32_t slot, n;
+    if (!load_request(a, req, &slot, &n)) return;
     const uint32_t* kept = a.kept + ((uint64_t)req * a.v.hkv + kv_head) * a.budget;
     const uint32_t* table = table_row(a.v, slot, a.v.layer);
+    uint32_t entries = a.budget;
+    for (uint32_t l = 0; l < a.levels; ++l) entries = lower_bound(kept, entries, entries);
     if (is_weights) {
-        move_runs<kUnroll>(a, kept, table, n, a.v.num_weight_pages, reinterpret_cast<uint32_t*>(a.page_weights), threadIdx.x,
-                           kThreads, true, [&](uint32_t page, uint32_t position) {
+        move_runs<kUnroll>(a, kept, table, n, entries, a.v.num_weight_pages, reinterpret_cast<uint32_t*>(a.page_weights),
+                           threadIdx.x, kThreads, true, [&](uint32_t page, uint32_t position) {
                                return weight_index(a.v, page, kv_head, page_place(a.v, position));
                            });
         return;
     }
     const uint32_t my_unit = blockIdx.x / a.group_stride * a.slice_units + threadIdx.x % a.slice_units;
-    move_runs<kUnroll>(a, kept, table, n, a.v.num_pages, static_cast<Unit*>(a.pages), threadIdx.x / a.slice_units,
+    move_runs<kUnroll>(a, kept, table, n, entries, a.v.num_pages, static_cast<Unit*>(a.pages), threadIdx.x / a.slice_units,
                        kThreads / a.slice_units, my_unit < a.line_units, [&](uint32_t page, uint32_t position) -> uint64_t {
                            const uint64_t line = (((uint64_t)page * 2 + kind) * a.v.hkv + kv_head) * a.v.tokens_per_page +
                                                  page_place(a.v, position);
                            return line * a.line_units + my_unit;
                        });
+}
+
+// The entries of one level: a workgroup takes kLevelEntries of a (request, KV head), whole lines of 2^log2_line units of
+// 16 bytes, K and V, eight units of a thread under way (78 us with 64 entries a workgroup, 86 with 128, 90 with 256).
+constexpr uint32_t kLevelEntries = 64, kLevelThreads = 256;
+__global__ __launch_bounds__(kLevelThreads) void compact_level_kernel(CompactArgs a, uint32_t level, uint32_t log2_line,
+                                                                      uint32_t chunks) {
+    const uint32_t kv_head = blockIdx.x / chunks % a.v.hkv, req = blockIdx.x / chunks / a.v.hkv;
+    const uint32_t base = blockIdx.x % chunks * kLevelEntries;
+    uint32_t slot, n;
+    if (!load_request(a, req, &slot, &n)) return;
+    const uint32_t* kept = a.kept + ((uint64_t)req * a.v.hkv + kv_head) * a.budget;
+    const uint32_t* table = table_row(a.v, slot, a.v.layer);
+    __shared__ uint64_t from_line[kLevelEntries], to_line[kLevelEntries];  // of K; all ones: nothing to move
+    __shared__ uint32_t moving;
+    constexpr uint64_t kNoLine = ~0ull;
+    const uint64_t kind_lines = (uint64_t)a.v.hkv * a.v.tokens_per_page;  // from a line of K to its line of V
+    if (threadIdx.x < kLevelEntries) {
+        const uint32_t i = base + threadIdx.x;
+        uint32_t at = i, src = i;
+        bool ours = i < a.budget;
+        for (uint32_t l = 0; l <= level; ++l) {
+            const uint32_t next = ours ? kept[at] : 0;
+            if (l == 0) src = next;
+            ours = ours && (l < level ? next > at && next < a.budget : next >= a.budget);
+            at = next;
+        }
+        from_line[threadIdx.x] = kNoLine;
+        if (ours) {
+            const bool there = src < n;
+            const uint32_t from = there ? table[page_index(a.v, src)] : kNoPage;
+            const uint32_t to = there ? table[page_index(a.v, i)] : kNoPage;
+            if (from < a.v.num_pages && to < a.v.num_pages) {
+                auto line_of = [&](uint32_t page, uint32_t p) {
+                    return ((uint64_t)page * 2 * a.v.hkv + kv_head) * a.v.tokens_per_page + page_place(a.v, p);
+                };
+                from_line[threadIdx.x] = line_of(from, src);
+                to_line[threadIdx.x] = line_of(to, i);
+            } else {
+                report_cache_range(a.status);
+            }
+            if (a.page_weights != nullptr) {
+                if (from < a.v.num_weight_pages && to < a.v.num_weight_pages)
+                    a.page_weights[weight_index(a.v, to, kv_head, page_place(a.v, i))] =
+                        a.page_weights[weight_index(a.v, from, kv_head, page_place(a.v, src))];
+                else
+                    report_cache_range(a.status);
+            }
+        }
+        const uint64_t any = __ballot(ours);
+        if (threadIdx.x == 0) moving = any != 0;
+    }
+    __syncthreads();
+    if (!moving) return;
+    unit_u32x4* data = static_cast<unit_u32x4*>(a.pages);
+    constexpr int kUnroll = 8;
+    const uint32_t units = kLevelEntries * 2 << log2_line;
+    for (uint32_t u0 = threadIdx.x; u0 < units; u0 += kLevelThreads * kUnroll) {
+        unit_u32x4 held[kUnroll];
+        uint64_t target[kUnroll];
+        bool moves[kUnroll];
+#pragma unroll
+        for (int u = 0; u < kUnroll; ++u) {
+            const uint32_t at = u0 + u * kLevelThreads, line = at >> log2_line, unit = at & ((1u << log2_line) - 1);
+            const uint32_t entry = min(line / 2, kLevelEntries - 1);
+            moves[u] = at < units && from_line[entry] != kNoLine;
+            const uint64_t kind = line % 2 ? kind_lines : 0;
+            held[u] = __builtin_nontemporal_load(data + (moves[u] ? ((from_line[entry] + kind) << log2_line) + unit : 0));
+            target[u] = ((to_line[entry] + kind) << log2_line) + unit;
+        }
+#pragma unroll
+        for (int u = 0; u < kUnroll; ++u)
+            if (moves[u]) data[target[u]] = held[u];
+    }
 }
 
 // Slices of a line: down to 128 bytes until there are four workgroups to a compute unit (32 requests of 1k-8k tokens cut
@@ -126,6 +230,20 @@ inline uint32_t compact_slices(uint64_t pairs, uint32_t line_bytes) {
     auto can_halve = [&](uint32_t least) { return line_bytes / (2 * slices) >= least; };
     while ((slices * pairs < 1024 && can_halve(128)) || (slices * pairs < 256 && can_halve(64))) slices *= 2;
     return slices;
+}
+
+// Levels that get launches of their own, where the runs have at most a workgroup for a compute unit: as long as a level
+// is likely to hold kLevelLeast entries, if the share of a request that is kept is spread evenly.  Without, with one, with
+// all of them: one request of 61001 cut to 30000 (4 heads of 256) 174, 115, 78 us; one of 131072 cut to 30000 (1 head of
+// 256) 147, 48, 33 us; two of 65536 cut to 50000 (4 heads of 128) 248, 216, 179 us, and 206 us with every level of a
+// thousand; four of 16000 cut to 8000 (8 heads of 128), 256 workgroups, 68 and 64 us.
+constexpr uint32_t kFewGroups = 256, kLevelLeast = 2048, kMostLevels = 4;
+inline uint32_t compact_levels(uint64_t groups, uint32_t budget, uint32_t max_cached) {
+    if (groups > kFewGroups || max_cached <= budget) return 0;
+    const double share = (double)budget / max_cached;
+    uint32_t levels = 0;
+    for (double left = budget; levels < kMostLevels && left * (1.0 - share) >= kLevelLeast; left *= share) ++levels;
+    return levels;
 }
 
 template <typename Unit>
@@ -181,12 +299,20 @@ extern "C" int psi_hip_kv_compact(psi_hip_ctx* ctx, const psi_hip_gqa_config* cf
     a.num_reqs = num_reqs;
     const uint64_t grid = stride * a.num_slices + (page_weights != nullptr ? pairs / 2 : 0);
     PSI_REQUIRE(grid <= 0x7fffffffull, "too many requests in one compaction");
+    a.levels = 0;
+    const uint64_t chunks = ((uint64_t)budget + kLevelEntries - 1) / kLevelEntries;
+    const uint64_t level_grid = chunks * (pairs / 2);
+    if (unit == 16 && (a.line_units & (a.line_units - 1)) == 0 && level_grid <= 0x7fffffffull)
+        a.levels = compact_levels(pairs * a.num_slices, budget, max_cached_tokens);
     DeviceGuard guard(ctx->device);
     LaunchScope scope(ctx, "kv_compact");
     a.group_stride = (uint32_t)stride;
     if (unit == 16) launch_compact<unit_u32x4>(ctx, a, (uint32_t)grid);
     else if (unit == 4) launch_compact<uint32_t>(ctx, a, (uint32_t)grid);
     else launch_compact<uint16_t>(ctx, a, (uint32_t)grid);
+    for (uint32_t level = a.levels; level-- > 0;)
+        hipLaunchKernelGGL(compact_level_kernel, dim3((uint32_t)level_grid), dim3(kLevelThreads), 0, ctx->stream, a, level,
+                           (uint32_t)__builtin_ctz(a.line_units), (uint32_t)chunks);
     PSI_HIP_CHECK(hipGetLastError());
     return PSI_HIP_OK;
 }

@@ -390,6 +390,18 @@ def test_compaction_of_a_long_request(psi, device):
     _compact(psi, device, [40000], 1, 128, "Bfloat16", 16, 1, 20000)
 
 
+@pytest.mark.parametrize("choose", [None, lambda rng, n: np.arange(n - 20000, n), lambda rng, n: np.arange(1, 20001),
+                                    lambda rng, n: np.arange(20000) if n % 2 else np.arange(20000) * 2 % n,
+                                    lambda rng, n: np.concatenate([np.arange(9001), np.arange(n - 10999, n)]),
+                                    lambda rng, n: np.sort(rng.permutation(np.arange(min(3, n - 20000), n))[:20000])],
+                         ids=["random", "tail", "one-on", "doubled", "both-ends", "sparse"])
+@pytest.mark.parametrize("d,page,ids,with_weights", [(64, 16, 1, True), (32, 5, 3, True), (128, 8, 2, False)])
+def test_compaction_of_few_long_requests(psi, device, choose, d, page, ids, with_weights):
+    """Entries that only wait for each other in a few steps, and chains of thousands of them."""
+    _compact(psi, device, [40000, 20000, 20001, 31111], 1, d, "Float16", page, ids, 20000, with_weights=with_weights,
+             choose=choose)
+
+
 def test_compaction_leaves_out_what_is_no_ascending_choice(psi, device):
     """Entries beyond the cached tokens, below their own index or on pages beyond the arena move nothing; the rest does."""
     wl = importlib_workloads(psi)
