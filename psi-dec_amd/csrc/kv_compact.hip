@@ -274,7 +274,7 @@ extern "C" int psi_hip_kv_compact(psi_hip_ctx* ctx, const psi_hip_gqa_config* cf
     if (rc != PSI_HIP_OK) return rc;
     PSI_REQUIRE(kv_pages && requests && kept, "compaction buffers must not be null");
     PSI_REQUIRE(num_reqs > 0, "a compaction needs requests");
-    PSI_REQUIRE(budget > 0, "the budget must be positive");
+    PSI_REQUIRE(budget > 0 && budget <= INT32_MAX, "the budget must be positive and below 2^31");
     PSI_REQUIRE((page_weights == nullptr) == (page_weights_bytes == 0), "accumulators need their size and vice versa");
     CompactArgs a;
     // without accumulators their bound does not matter

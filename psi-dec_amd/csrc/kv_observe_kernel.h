@@ -138,11 +138,10 @@ __global__ __launch_bounds__(64 * kWaves, kWaves / 4) void observe_kernel(Observ
             uint4 value[kStage];
 #pragma unroll
             for (int u = 0; u < kStage; ++u) {
-                const uint32_t i = i0 + u * kThreads, c = c0 + i / kChunks;
-                const bool there = i < units && c < columns;
+                // (columns that fill up the last block repeat the last one: what is finite there stays finite)
+                const uint32_t i = i0 + u * kThreads, c = min(c0 + i / kChunks, columns - 1);
                 const uint64_t q_row = (uint64_t)(r.q_begin + c / a.group) * a.hq + kv_head * a.group + c % a.group;
-                value[u] = *reinterpret_cast<const uint4*>(q + (there ? q_row * D + i % kChunks * 8 : 0));
-                if (!there) value[u] = make_uint4(0, 0, 0, 0);
+                value[u] = *reinterpret_cast<const uint4*>(q + q_row * D + i % kChunks * 8);
             }
 #pragma unroll
             for (int u = 0; u < kStage; ++u) {

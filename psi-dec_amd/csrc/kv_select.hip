@@ -359,7 +359,7 @@ extern "C" int psi_hip_kv_select_kept(psi_hip_ctx* ctx, const psi_hip_gqa_config
     if (rc != PSI_HIP_OK) return rc;
     PSI_REQUIRE(page_weights && requests && kept, "selection buffers must not be null");
     PSI_REQUIRE(num_reqs > 0, "a selection needs requests");
-    PSI_REQUIRE(budget > 0, "the budget must be positive");
+    PSI_REQUIRE(budget > 0 && budget <= INT32_MAX, "the budget must be positive and below 2^31");
     PSI_REQUIRE((uint64_t)num_first + num_recent <= budget, "the tokens that are always kept exceed the budget: %u + %u > %u",
                 num_first, num_recent, budget);
     SelectArgs a;

@@ -112,8 +112,10 @@ class GQAKVObserveKernels:
                decay: float = 1.0):
         """Adds the windows' weights to `page_weights`; `q`: [query tokens][Q heads][head_dim], rotated."""
         _check_page_weights(page_weights, self.device)
-        if q.numel() < plan.num_q_tokens * self.config.num_q_heads * self.config.head_dim or not q.is_contiguous():
-            raise ValueError("q: contiguous rows for every planned query token are wanted")
+        if (q.numel() < plan.num_q_tokens * self.config.num_q_heads * self.config.head_dim or not q.is_contiguous() or
+                q.element_size() != self.config.dtype.item_size() or q.device != self.device.torch_device):
+            raise ValueError("q: contiguous rows of the cache's type on the kernels' device are wanted, one for every "
+                             "planned query token")
         L.check(self.device.lib.psi_hip_kv_observe_weights(
             self.device.ctx, ctypes.byref(self._cfg), ctypes.byref(self._layout), _ptr(q), plan.num_q_tokens,
             _ptr(kv_pages), _nbytes(kv_pages), _ptr(page_ids), _ptr(plan.windows), plan.num_windows, plan.max_window,
@@ -181,7 +183,8 @@ class GQAKVEvictionKernels:
 
         if page_weights is not None:
             _check_page_weights(page_weights, self.device)
-        if kept.dtype != torch.int32 or not kept.is_contiguous() or kept.numel() != plan.kept.numel():
+        if (kept.dtype != torch.int32 or not kept.is_contiguous() or kept.numel() != plan.kept.numel() or
+                kept.device != self.device.torch_device):
             raise ValueError("kept: the contiguous int32 [requests][KV heads][budget] of a selection is wanted")
         L.check(self.device.lib.psi_hip_kv_compact(
             self.device.ctx, ctypes.byref(self._cfg), ctypes.byref(self._layout), _ptr(kv_pages), _nbytes(kv_pages),

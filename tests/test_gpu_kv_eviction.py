@@ -230,6 +230,24 @@ def test_observation_ignores_what_lies_behind_the_context(psi, device):
     _assert_weights(_observe(psi, device, w, acc, [0, 0], 1.0).cpu().numpy(), exp, bound)
 
 
+@pytest.mark.parametrize("hq,hkv,d", [(3, 3, 256), (10, 2, 128), (4, 2, 64)])
+def test_observation_of_a_key_that_nothing_can_attend_to(psi, device, hq, hkv, d):
+    """A key whose logits are -inf for every query (an infinite element, all queries positive) receives nothing; the
+    weights of the others sum to one per query, also where the queries do not fill a block of columns."""
+    wl = importlib_workloads(psi)
+    w = wl.make_workload(27, [150], hq, hkv, d, psi.Dtype.Bfloat16, 16, q_lens=[5], **LAYERS)
+    w.q = np.where((w.q & 0x7fff) == 0, 0x3f80, w.q & 0x7fff).astype(np.uint16)
+    rows = page_rows(w, 0)
+    w.pages[rows[33 // 16], 0, :, 33 % 16, 7] = 0xff80
+    acc = np.full((w.num_pages, hkv, 16), 3.0, np.float32)
+    got = _observe(psi, device, w, acc, [0], 1.0).cpu().numpy()
+    p = np.arange(150)
+    mine = got[rows[p // 16], :, p % 16]
+    assert np.isfinite(mine).all() and (mine[33] == 0.0).all()
+    # 150 weights of 5 * group queries, each a few roundings of exp2 and of a normaliser of 150 terms
+    assert np.abs(mine.sum(axis=0) / (5 * hq // hkv) - 1.0).max() <= 2.0 ** -24 * (2 * 150 + 5 * (hq // hkv) + 64)
+
+
 def test_observation_leaves_out_pages_beyond_the_arena(psi, device):
     wl = importlib_workloads(psi)
     w = wl.make_workload(24, [64, 48], 24, 4, 256, psi.Dtype.Bfloat16, 16, q_lens=4, **LAYERS)
