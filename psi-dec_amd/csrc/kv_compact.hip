@@ -57,17 +57,25 @@ __device__ __forceinline__ uint32_t lower_bound(const uint32_t* values, uint32_t
 }
 
 // The runs of one (request, KV head, slice): a workgroup takes `per_step` lines at a time, a unit a lane, kUnroll
-// steps a run.  What a run's lines need is asked for ahead, a link of the chain per run: the kept positions two runs
-// ahead, the page IDs one run ahead, then the lines, so that a run waits for memory once.  Entries that move nothing read
-// the first unit of the array in place of a line, so that the loads of a run stand without branches between them.
-template <int kUnroll, typename Unit, typename Index>
+// steps a run.  No run writes what a later one reads, so the lines of the next run are asked for before those of this one
+// have come; what they need is asked for ahead of that, a link of the chain per run: the kept positions three runs ahead,
+// the page IDs two runs ahead.  (Loads come back in the order of their issue: lines are asked for after the page IDs and
+// kept positions of an iteration, which the next one waits for first.)  Entries that move nothing read the first unit of
+// the array in place of a line, so that the loads of a run stand without branches between them.
+template <bool kStream, int kUnroll, typename Unit, typename Index>
 __device__ __forceinline__ void move_runs(const CompactArgs& a, const uint32_t* kept, const uint32_t* table, uint32_t n,
                                           uint32_t entries, uint32_t num_pages, Unit* data, uint32_t my_line,
                                           uint32_t per_step, bool in_line, Index index) {
     const uint32_t per_run = per_step * kUnroll;
-    uint32_t src[kUnroll], src_next[kUnroll], from[kUnroll], to[kUnroll];
+    struct Places {
+        uint32_t src[kUnroll], from[kUnroll], to[kUnroll];
+    };
+    struct Lines {
+        Unit held[kUnroll];
+        uint32_t to[kUnroll];  // kNoPage: nothing is moved
+    };
     auto entry = [&](uint32_t base, int u) -> uint32_t { return base + u * per_step + my_line; };
-    auto fetch_kept = [&](uint32_t base, uint32_t (&out)[kUnroll]) {
+    auto fetch_kept = [&](uint32_t base, uint32_t (&out)[kUnroll]) __attribute__((always_inline)) {
 #pragma unroll
         for (int u = 0; u < kUnroll; ++u) {
             const uint32_t i = entry(base, u);
@@ -76,50 +84,66 @@ __device__ __forceinline__ void move_runs(const CompactArgs& a, const uint32_t* 
             out[u] = there ? k : i;  // an entry that stays where it is moves nothing
         }
     };
-    auto fetch_pages = [&](uint32_t base, const uint32_t (&at)[kUnroll]) {
+    auto fetch_pages = [&](uint32_t base, const uint32_t (&at)[kUnroll], Places& p) __attribute__((always_inline)) {
 #pragma unroll
         for (int u = 0; u < kUnroll; ++u) {
             const uint32_t i = entry(base, u);
             const bool moves = at[u] > i && at[u] < n;  // (n's positions have entries in the table)
-            from[u] = table[moves ? page_index(a.v, at[u]) : 0];
-            to[u] = table[moves ? page_index(a.v, i) : 0];
-            if (!moves || from[u] >= num_pages || to[u] >= num_pages) from[u] = to[u] = kNoPage;
+            p.src[u] = at[u];
+            p.from[u] = table[moves ? page_index(a.v, at[u]) : 0];
+            p.to[u] = table[moves ? page_index(a.v, i) : 0];
+            if (!moves) p.to[u] = kNoPage;
         }
     };
-    fetch_kept(0, src);
-    fetch_kept(per_run, src_next);
-    fetch_pages(0, src);
-    for (uint32_t base = 0; base < entries; base += per_run) {
-        Unit held[kUnroll];
-        uint64_t target[kUnroll];
-        uint32_t moves = 0;
+    auto fetch_lines = [&](uint32_t base, const Places& p, Lines& l) __attribute__((always_inline)) {
 #pragma unroll
         for (int u = 0; u < kUnroll; ++u) {
-            const uint32_t i = entry(base, u);
-            const bool found = from[u] != kNoPage;
+            const bool found = p.from[u] < num_pages && p.to[u] < num_pages;
             // beyond the cached tokens or the arena, or not ascending: nothing is moved for this entry
-            if (!found && src[u] != i) report_cache_range(a.status);
-            held[u] = __builtin_nontemporal_load(data + (found ? index(from[u], src[u]) : 0));
-            target[u] = index(to[u], i);
-            moves |= (found ? 1u : 0u) << u;
+            if (!found && p.src[u] != entry(base, u)) report_cache_range(a.status);
+            const Unit* from = data + (found ? index(p.from[u], p.src[u]) : 0);
+            l.held[u] = kStream ? __builtin_nontemporal_load(from) : *from;
+            l.to[u] = found ? p.to[u] : kNoPage;
         }
-        fetch_pages(base + per_run, src_next);
+    };
+    auto store_lines = [&](uint32_t base, Lines& l) __attribute__((always_inline)) {
 #pragma unroll
-        for (int u = 0; u < kUnroll; ++u) src[u] = src_next[u];
-        fetch_kept(base + 2 * per_run, src_next);
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // the run has been read ...
-        __syncthreads();                                  // ... by every wave before any of it is written
+        for (int u = 0; u < kUnroll; ++u) asm volatile("" : "+v"(l.held[u]));  // the run has been read ...
+        asm volatile("" ::: "memory");
+        __builtin_amdgcn_s_barrier();  // ... by every wave before any of it is written
+        asm volatile("" ::: "memory");
 #pragma unroll
         for (int u = 0; u < kUnroll; ++u)
-            if (moves >> u & 1) data[target[u]] = held[u];
+            if (l.to[u] != kNoPage) data[index(l.to[u], entry(base, u))] = l.held[u];
+    };
+    if (entries == 0) return;
+    uint32_t at[kUnroll];
+    Places even, odd;
+    Lines first, second;
+    fetch_kept(0, at);
+    fetch_pages(0, at, even);
+    fetch_kept(per_run, at);
+    fetch_pages(per_run, at, odd);
+    fetch_kept(2 * per_run, at);
+    fetch_lines(0, even, first);
+    for (uint32_t base = 0; base < entries; base += 2 * per_run) {
+        fetch_pages(base + 2 * per_run, at, even);
+        fetch_kept(base + 3 * per_run, at);
+        fetch_lines(base + per_run, odd, second);
+        store_lines(base, first);
+        if (base + per_run >= entries) break;
+        fetch_pages(base + 3 * per_run, at, odd);
+        fetch_kept(base + 4 * per_run, at);
+        fetch_lines(base + 2 * per_run, even, first);
+        store_lines(base + per_run, second);
     }
 }
 
 // One workgroup per (slice, request, KV head, K | V), then one per (request, KV head) for the accumulators; slice_units
 // divides kThreads.  The slices of a line are a multiple of eight workgroups apart, so that they go to one XCD and share
 // in its L2 the lines of memory that a slice of less than 128 bytes reads a part of.
-template <typename Unit, int kThreads, int kUnroll>
-__global__ __launch_bounds__(kThreads) void compact_kernel(CompactArgs a) {
+template <typename Unit, int kThreads, int kUnroll, bool kStream>
+__global__ __launch_bounds__(kThreads, kThreads == 1024 ? 4 : 8) void compact_kernel(CompactArgs a) {
     const uint32_t line_groups = a.group_stride * a.num_slices;
     const bool is_weights = blockIdx.x >= line_groups;
     const uint32_t pair = is_weights ? (blockIdx.x - line_groups) * 2 : blockIdx.x % a.group_stride;
@@ -132,14 +156,14 @@ __global__ __launch_bounds__(kThreads) void compact_kernel(CompactArgs a) {
     uint32_t entries = a.budget;
     for (uint32_t l = 0; l < a.levels; ++l) entries = lower_bound(kept, entries, entries);
     if (is_weights) {
-        move_runs<kUnroll>(a, kept, table, n, entries, a.v.num_weight_pages, reinterpret_cast<uint32_t*>(a.page_weights),
+        move_runs<kStream, kUnroll>(a, kept, table, n, entries, a.v.num_weight_pages, reinterpret_cast<uint32_t*>(a.page_weights),
                            threadIdx.x, kThreads, true, [&](uint32_t page, uint32_t position) {
                                return weight_index(a.v, page, kv_head, page_place(a.v, position));
                            });
         return;
     }
     const uint32_t my_unit = blockIdx.x / a.group_stride * a.slice_units + threadIdx.x % a.slice_units;
-    move_runs<kUnroll>(a, kept, table, n, entries, a.v.num_pages, static_cast<Unit*>(a.pages), threadIdx.x / a.slice_units,
+    move_runs<kStream, kUnroll>(a, kept, table, n, entries, a.v.num_pages, static_cast<Unit*>(a.pages), threadIdx.x / a.slice_units,
                        kThreads / a.slice_units, my_unit < a.line_units, [&](uint32_t page, uint32_t position) -> uint64_t {
                            const uint64_t line = (((uint64_t)page * 2 + kind) * a.v.hkv + kv_head) * a.v.tokens_per_page +
                                                  page_place(a.v, position);
@@ -223,21 +247,21 @@ __global__ __launch_bounds__(kLevelThreads) void compact_level_kernel(CompactArg
 
 // Slices of a line: down to 128 bytes until there are four workgroups to a compute unit (32 requests of 1k-8k tokens cut
 // to 1024, 4 heads of 256: 86 us with whole lines, 48 us with 128 bytes, which is 5.4 TB/s read and written); where that
-// leaves compute units without one, down to 64 bytes (one request of 61001 tokens cut to 30000, 4 heads of 256: 206 us
-// with 128 bytes, 175 us with 64, 168 us with 32; four of 16000 cut to 8000, 8 heads of 128: 74, 69 and 118 us).
+// leaves compute units without one, down to 32 bytes (one request of 8000 cut to 4000, 2 heads of 256: 14.4 us, 15.3 with
+// 64 bytes; two of 65536 cut to 50000, 4 heads of 128: 164 and 172 us).
 inline uint32_t compact_slices(uint64_t pairs, uint32_t line_bytes) {
     uint32_t slices = 1;
     auto can_halve = [&](uint32_t least) { return line_bytes / (2 * slices) >= least; };
-    while ((slices * pairs < 1024 && can_halve(128)) || (slices * pairs < 256 && can_halve(64))) slices *= 2;
+    while ((slices * pairs < 1024 && can_halve(128)) || (slices * pairs < 256 && can_halve(32))) slices *= 2;
     return slices;
 }
 
-// Levels that get launches of their own, where the runs have at most a workgroup for a compute unit: as long as a level
-// is likely to hold kLevelLeast entries, if the share of a request that is kept is spread evenly.  Without, with one, with
-// all of them: one request of 61001 cut to 30000 (4 heads of 256) 174, 115, 78 us; one of 131072 cut to 30000 (1 head of
-// 256) 147, 48, 33 us; two of 65536 cut to 50000 (4 heads of 128) 248, 216, 179 us, and 206 us with every level of a
-// thousand; four of 16000 cut to 8000 (8 heads of 128), 256 workgroups, 68 and 64 us.
-constexpr uint32_t kFewGroups = 256, kLevelLeast = 2048, kMostLevels = 4;
+// Levels that get launches of their own, where the runs have a workgroup for every second compute unit at most: as long
+// as a level is likely to hold kLevelLeast entries, if the share of a request that is kept is spread evenly.  Without, with
+// one, with all of them: one request of 61001 cut to 30000 (4 heads of 256) 126, 78, 72 us; one of 131072 cut to 30000 (1
+// head of 256) 76, 36, 31 us; two of 65536 cut to 50000 (4 heads of 128) 197, 181, 164 us (seven levels cost what they
+// gain); four of 16000 cut to 8000 (8 heads of 128), 256 workgroups, 61 us either way.
+constexpr uint32_t kFewGroups = 128, kLevelLeast = 2048, kMostLevels = 4;
 inline uint32_t compact_levels(uint64_t groups, uint32_t budget, uint32_t max_cached) {
     if (groups > kFewGroups || max_cached <= budget) return 0;
     const double share = (double)budget / max_cached;
@@ -248,13 +272,14 @@ inline uint32_t compact_levels(uint64_t groups, uint32_t budget, uint32_t max_ca
 
 template <typename Unit>
 static void launch_compact(psi_hip_ctx* ctx, const CompactArgs& a, uint32_t grid) {
-    // Many workgroups: short runs, several to a compute unit (55 us with four units a lane, 48 us with two on the 32
-    // requests above).  Few: long runs, which a wait for memory each costs less of (one of 61001: 378 us with 512 threads
-    // and two units, 216 us with 1024 and four, in 128-byte slices).
+    // Many workgroups: a unit a lane, four workgroups to a compute unit, streaming loads (the 32 requests above: 48 us; 57
+    // with two units, whose registers leave room for three; 65 with ordinary loads, 65 with the other launch).  Few: long
+    // runs and ordinary loads, as slices share lines of memory (one of 8000 cut to 4000: 14.4 us, 18.9 with the other
+    // launch; four of 16000 cut to 8000: 61 and 76 us).
     if (grid >= 512)
-        hipLaunchKernelGGL((compact_kernel<Unit, 512, 2>), dim3(grid), dim3(512), 0, ctx->stream, a);
+        hipLaunchKernelGGL((compact_kernel<Unit, 512, 1, true>), dim3(grid), dim3(512), 0, ctx->stream, a);
     else
-        hipLaunchKernelGGL((compact_kernel<Unit, 1024, 4>), dim3(grid), dim3(1024), 0, ctx->stream, a);
+        hipLaunchKernelGGL((compact_kernel<Unit, 1024, 4, false>), dim3(grid), dim3(1024), 0, ctx->stream, a);
 }
 
 }  // namespace psi
