@@ -79,9 +79,15 @@ __device__ __forceinline__ void join_rows(const ObserveArgs& a, uint32_t first, 
         for (uint32_t u = 0; u < kAhead; ++u) join_states(part[u], m, s);
     }
 }
-__device__ __forceinline__ float join_column(const ObserveArgs& a, const ObserveRow& r, uint32_t kv_head, uint32_t column) {
+// The same by `parts` adjacent lanes (a power of two), each of which gets the normaliser of the column.
+__device__ __forceinline__ float join_column(const ObserveArgs& a, const ObserveRow& r, uint32_t kv_head, uint32_t column,
+                                             uint32_t part, uint32_t parts) {
     float m = kEmptyMax, s = 0.0f;
-    join_rows(a, r.row_begin, r.row_end, 1, kv_head, column, &m, &s);
+    join_rows(a, r.row_begin + part, r.row_end, parts, kv_head, column, &m, &s);
+    for (uint32_t off = parts / 2; off > 0; off /= 2) {
+        const float2 other = make_float2(__shfl_xor(m, off, 64), __shfl_xor(s, off, 64));
+        join_states(other, &m, &s);
+    }
     return lse_of_state(m, s);
 }
 

@@ -21,9 +21,9 @@
 
 namespace psi {
 
-// Normalisers are joined inside the second pass as long as (rows of a window) * (columns) stays within this: at 160 and
-// 1460 that saves the 2 us of a launch (13 for 15 us and 66 for 68 us in all); at 10240 the two come out even, and
-// beyond, every workgroup would repeat a join that grows with the row count.
+// Normalisers are joined inside the second pass as long as (rows of a window) * (columns) stays within this, which saves
+// a launch (at 104: 13.2 for 15.7 us in all, at 1460: 59 for 62, at 6656: 10.9 for 13.3); at 10240 the two come out even,
+// and at 30016 (55 us in all) repeating the join in every workgroup costs 4 us.
 constexpr uint64_t kFusedJoins = 8192;
 
 template <int kCtrl>
@@ -153,11 +153,20 @@ __global__ __launch_bounds__(64 * kWaves, kWaves / 4) void observe_kernel(Observ
         for (uint32_t i = tid; i < blocks * 16; i += kThreads) {
             const uint32_t c = c0 + i;
             last_lds[i] = c < columns ? (int)min(r.position + c / a.group, key_end - 1) : -1;
-            if constexpr (kSum)
+            if (kSum && (a.lse != nullptr || c >= columns))
                 lse_lds[i] = c >= columns ? INFINITY
-                             : a.lse != nullptr
-                                 ? a.lse[(uint64_t)(r.q_begin + c / a.group) * a.hq + kv_head * a.group + c % a.group]
-                                 : join_column(a, r, kv_head, c);
+                                          : a.lse[(uint64_t)(r.q_begin + c / a.group) * a.hq + kv_head * a.group + c % a.group];
+        }
+        if (kSum && a.lse == nullptr) {
+            // a column's rows are shared out among the lanes that its neighbours leave (8 tokens of 13234, 208 rows: 10.9
+            // us for 19.8 with a lane a column)
+            const uint32_t rows = r.row_end - min(r.row_begin, r.row_end);
+            uint32_t parts = 1;
+            while (parts < 64 && 2 * parts * count <= kThreads && 8 * parts < rows) parts *= 2;
+            for (uint32_t i = tid; i < count * parts; i += kThreads) {
+                const float lse = join_column(a, r, kv_head, c0 + i / parts, i % parts, parts);
+                if (i % parts == 0) lse_lds[i / parts] = lse;
+            }
         }
         if constexpr (!kSum)
             for (uint32_t i = lane; i < blocks * 16; i += 64) state_lds[wave][i] = make_float2(kEmptyMax, 0.0f);
