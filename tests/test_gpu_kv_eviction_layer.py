@@ -256,3 +256,52 @@ def test_pages_beyond_32_bit_offsets(psi, device):
     for a, b in zip(got, exp):
         assert np.array_equal(a, b)
     assert not acc[:first].any()
+
+
+def test_long_selection_and_compaction_captured(psi, device):
+    """The forms of several launches (a selection in chunks, a compaction in levels) in a graph, replayed."""
+    import torch
+
+    wl = importlib_workloads(psi)
+    w = wl.make_workload(91, [20001, 17000], 1, 1, 64, psi.Dtype.Float16, 16, **LAYERS)
+    stream = torch.cuda.Stream()
+    dev = psi.Device(0, stream)
+    evict = psi.GQAKVEvictionKernels(dev, _config(psi, w), 9000, 4, 8)
+    with torch.cuda.stream(stream):
+        plan = evict.prepare(w.req_slots, w.context_lens)
+        ids, start = dev.from_numpy(w.page_ids), (dev.from_numpy(w.pages.reshape(-1)), dev.from_numpy(_weights(w)))
+        pages, acc = (t.clone() for t in start)
+
+    def step():
+        evict.invoke_compact(plan, evict.invoke_select(plan, acc, ids, w.layer), pages, acc, ids, w.layer)
+
+    def results():
+        dev.sync()
+        return [t.view(torch.uint8).cpu().numpy().copy() for t in (pages, acc, plan.kept)]
+
+    with torch.cuda.stream(stream):
+        step()
+    exp = results()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=stream):
+        step()
+    for _ in range(3):
+        with torch.cuda.stream(stream):
+            pages.copy_(start[0])
+            acc.copy_(start[1])
+            graph.replay()
+            got = results()
+            torch.randn(1 << 18, device="cuda").sum().item()
+        for a, b in zip(got, exp):
+            assert np.array_equal(a, b)
+    # the plain form of what was kept and moved
+    from eviction_util import compacted, kept_positions
+
+    host_pages, host_acc = w.pages.copy(), _weights(w)
+    for r, n in enumerate(w.context_lens):
+        rows, p = page_rows(w, r), np.arange(int(n))
+        keep = [kept_positions(host_acc[rows[p // 16], 0, p % 16], int(n), 9000, 4, 8)]
+        assert np.array_equal(exp[2].view(np.int32).reshape(2, 9000)[r], keep[0])
+        host_pages, host_acc = compacted(host_pages, host_acc, rows, keep, 16)
+    assert exp[0].tobytes() == host_pages.tobytes() and exp[1].tobytes() == host_acc.tobytes()
+    dev.close()

@@ -138,6 +138,16 @@ def test_null_arguments_are_refused_before_a_gpu_is_touched(psi):
     assert b"must not be null" in lib.psi_hip_last_error()
 
 
+def test_layer_call_refuses_missing_weights_and_contexts(psi):
+    lib, L = psi.load(), psi._lib
+    cfg, inp, weights = L.LayerConfigStruct(), L.LayerInputStruct(), L.KVWeightsStruct()
+    assert lib.psi_hip_gqa_layer_record_weights(None, ctypes.byref(cfg), ctypes.byref(inp), None) == L.ERR_INVALID_ARGUMENT
+    assert b"weights must not be null" in lib.psi_hip_last_error()
+    assert lib.psi_hip_gqa_layer_record_weights(None, ctypes.byref(cfg), ctypes.byref(inp),
+                                                ctypes.byref(weights)) == L.ERR_INVALID_ARGUMENT
+    assert b"ctx must not be null" in lib.psi_hip_last_error()
+
+
 def test_kernel_classes_refuse_budgets_that_do_not_hold_what_is_always_kept(psi):
     for budget, first, recent in ((0, 0, 0), (4, 3, 2), (4, -1, 0)):
         with pytest.raises(ValueError, match="budget"):
