@@ -242,20 +242,26 @@ __global__ __launch_bounds__(kSelectThreads) void select_row_kernel(SelectArgs a
     emit<kQuads>(a, emit_lds, key, 0, st.prefix, st.remaining, 0, 0, kept);
 }
 
-// Longer rows: a workgroup per (row, chunk of 8192 positions) and a launch per digit.  Each launch adds up the counters
+// Longer rows: a workgroup per (row, chunk of 4096 or 8192 positions) and a launch per digit.  Each launch adds up the counters
 // that the one before left for every chunk of the row, which gives the digit's value and, from the chunks ahead, the
 // number of kept positions before this chunk's first; so nothing is cleared or added atomically in memory.
-constexpr int kChunkQuads = 2;
-constexpr uint32_t kChunkKeys = 4 * kChunkQuads * kSelectThreads;
+constexpr uint32_t chunk_keys(int quads) { return 4 * quads * kSelectThreads; }
 struct ChunkState {
     uint32_t prefix, remaining, gt_before, unused;
 };
-__host__ __device__ inline uint64_t select_chunks(uint32_t max_cached) { return ((uint64_t)max_cached + kChunkKeys - 1) / kChunkKeys; }
+inline uint64_t select_chunks(uint32_t max_cached, int quads) {
+    return ((uint64_t)max_cached + chunk_keys(quads) - 1) / chunk_keys(quads);
+}
+// Chunks of 4096 while those of 8192 would leave half of the compute units without one (4 requests of 131072 on 2 heads: 28
+// us for 30; 6 of up to 38290 on 4 heads: 25 for 29), which costs a chunk twice the counters to add up (40 requests of
+// 30000 on 8 heads: 128 us for 100).
+inline int chunk_quads(uint64_t rows, uint32_t max_cached) { return rows * select_chunks(max_cached, 2) <= 128 ? 1 : 2; }
 
 // kPass 0 .. 2: counts digit kPass; kPass 3: writes the positions.
-template <int kPass>
-__global__ __launch_bounds__(kSelectThreads) void select_chunk_kernel(SelectArgs a, uint32_t num_chunks, uint32_t* hists,
+template <int kPass, int kChunkQuads>
+__global__ __launch_bounds__(kSelectThreads) void select_chunk_kernel(SelectArgs a, uint32_t num_chunks, uint16_t* hists,
                                                                       ChunkState* states) {
+    constexpr uint32_t kChunkKeys = chunk_keys(kChunkQuads);
     __shared__ __attribute__((aligned(16))) uint32_t hist[kCopies * kBins];
     __shared__ BinSearch search;
     __shared__ EmitLds emit_lds;
@@ -286,17 +292,17 @@ __global__ __launch_bounds__(kSelectThreads) void select_chunk_kernel(SelectArgs
         const uint32_t at = kBins - 2 - 2 * tid;
         constexpr uint32_t kAhead = 16;  // chunks asked for at a time
         for (uint32_t c0 = 0; c0 < row_chunks; c0 += kAhead) {
-            uint2 v[kAhead];
+            uint32_t v[kAhead];
 #pragma unroll
             for (uint32_t u = 0; u < kAhead; ++u)
-                v[u] = c0 + u < row_chunks ? *reinterpret_cast<const uint2*>(bins_of(kPass - 1, c0 + u) + at) : make_uint2(0, 0);
+                v[u] = c0 + u < row_chunks ? *reinterpret_cast<const uint32_t*>(bins_of(kPass - 1, c0 + u) + at) : 0;
 #pragma unroll
             for (uint32_t u = 0; u < kAhead; ++u) {
-                low += v[u].x;
-                high += v[u].y;
+                low += v[u] & 0xffff;
+                high += v[u] >> 16;
                 if (c0 + u < chunk) {
-                    low_ahead += v[u].x;
-                    high_ahead += v[u].y;
+                    low_ahead += v[u] & 0xffff;
+                    high_ahead += v[u] >> 16;
                 }
             }
         }
@@ -318,15 +324,15 @@ __global__ __launch_bounds__(kSelectThreads) void select_chunk_kernel(SelectArgs
         __syncthreads();
         count_digits<kChunkQuads>(hist, key, kPass, st.prefix);
         __syncthreads();
-        uint32_t* out = bins_of(kPass, chunk);
-        for (uint32_t b = tid; b < kBins; b += kSelectThreads) out[b] = bin_count(hist, b);
+        static_assert(kBins == 2 * kSelectThreads && kChunkKeys < 65536, "two counters of 16 bits a thread");
+        reinterpret_cast<uint32_t*>(bins_of(kPass, chunk))[tid] = bin_count(hist, 2 * tid) | bin_count(hist, 2 * tid + 1) << 16;
     } else {
         emit<kChunkQuads>(a, emit_lds, key, first, st.prefix, st.remaining, gt_before, equal_before, kept);
     }
 }
 
 // Rows of up to this many positions go to one workgroup each: what its registers hold.  One launch of it takes 17 us at
-// 16384 positions and 11 at 8192, the four launches over chunks 27 at either (32 sequences: 19 and 12 against 32 and 29).
+// 16384 positions and 11 at 8192, the four launches over chunks 23 and 22 (32 sequences: 19 and 12 against 31 and 25).
 constexpr uint32_t kRowPositions = 16384;
 
 }  // namespace psi
@@ -340,8 +346,9 @@ extern "C" int psi_hip_kv_select_scratch_bytes(const psi_hip_gqa_config* cfg, ui
     if (rc != PSI_HIP_OK) return rc;
     PSI_REQUIRE(out_bytes != nullptr, "out pointer must not be null");
     PSI_REQUIRE(num_reqs > 0, "a selection needs requests");
-    const uint64_t chunks = (uint64_t)num_reqs * g.hkv * select_chunks(max_cached_tokens);
-    *out_bytes = max_cached_tokens <= kRowPositions ? 0 : chunks * (kDigits * kBins * 4 + sizeof(ChunkState));
+    const uint64_t rows = (uint64_t)num_reqs * g.hkv;
+    const uint64_t chunks = rows * select_chunks(max_cached_tokens, chunk_quads(rows, max_cached_tokens));
+    *out_bytes = max_cached_tokens <= kRowPositions ? 0 : chunks * (kDigits * kBins * 2 + sizeof(ChunkState));
     return PSI_HIP_OK;
 }
 
@@ -391,15 +398,19 @@ extern "C" int psi_hip_kv_select_kept(psi_hip_ctx* ctx, const psi_hip_gqa_config
     } else if (max_cached_tokens <= kRowPositions) {
         hipLaunchKernelGGL(select_row_kernel<4>, dim3(rows), threads, 0, ctx->stream, a);
     } else {
-        const uint64_t chunks = select_chunks(max_cached_tokens), grid = rows * chunks;
+        const int quads = chunk_quads(rows, max_cached_tokens);
+        const uint64_t chunks = select_chunks(max_cached_tokens, quads), grid = rows * chunks;
         PSI_REQUIRE(grid <= 0x7fffffffull, "too many requests of this length in one selection");
-        uint32_t* hists = static_cast<uint32_t*>(scratch);
+        uint16_t* hists = static_cast<uint16_t*>(scratch);
         ChunkState* states = reinterpret_cast<ChunkState*>(hists + grid * kDigits * kBins);
         const dim3 blocks((uint32_t)grid);
-        hipLaunchKernelGGL(select_chunk_kernel<0>, blocks, threads, 0, ctx->stream, a, (uint32_t)chunks, hists, states);
-        hipLaunchKernelGGL(select_chunk_kernel<1>, blocks, threads, 0, ctx->stream, a, (uint32_t)chunks, hists, states);
-        hipLaunchKernelGGL(select_chunk_kernel<2>, blocks, threads, 0, ctx->stream, a, (uint32_t)chunks, hists, states);
-        hipLaunchKernelGGL(select_chunk_kernel<3>, blocks, threads, 0, ctx->stream, a, (uint32_t)chunks, hists, states);
+        auto launch = [&](auto kernel) {
+            hipLaunchKernelGGL(kernel, blocks, threads, 0, ctx->stream, a, (uint32_t)chunks, hists, states);
+        };
+        launch(quads == 1 ? select_chunk_kernel<0, 1> : select_chunk_kernel<0, 2>);
+        launch(quads == 1 ? select_chunk_kernel<1, 1> : select_chunk_kernel<1, 2>);
+        launch(quads == 1 ? select_chunk_kernel<2, 1> : select_chunk_kernel<2, 2>);
+        launch(quads == 1 ? select_chunk_kernel<3, 1> : select_chunk_kernel<3, 2>);
     }
     PSI_HIP_CHECK(hipGetLastError());
     return PSI_HIP_OK;

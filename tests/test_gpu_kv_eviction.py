@@ -330,7 +330,8 @@ def test_selection(psi, device, values, budget, first, recent):
 
 
 @pytest.mark.parametrize("lens,hkv,page,ids", [([70001, 65536, 300], 2, 16, 1), ([40000], 8, 8, 4), ([9000, 33], 3, 5, 2),
-                                              ([16384, 4097, 8192], 2, 16, 1), ([16385, 24576, 24577, 8193, 5], 2, 16, 1),
+                                              ([16384, 4097, 8192], 2, 16, 1), (range(17000, 19000, 300), 8, 16, 1),
+                                              ([16385, 24576, 24577, 8193, 5], 2, 16, 1),
                                               ([20011, 12289], 2, 7, 1)])
 @pytest.mark.parametrize("values", ["softmax", "ties", "equal"])
 def test_selection_of_long_requests(psi, device, lens, hkv, page, ids, values):
