@@ -9,7 +9,7 @@
 //
 // A result lane holds 4 * kTiles keys of one column: the maximum and sum of a column (first pass) are reduced over the
 // lane and then over the four lanes of the column, the weights of a key (second pass) over the columns of a lane first
-// and over the lanes once per turn.
+// and over the lanes once per turn.  Where waves share the columns of a key, their sums meet in LDS.
 //
 // Measured: 8 prompts of 1k-8k (bf16, D 256, 32 tokens, 24 heads over 4) 58 us for two walks of 75 MB and 2 * 14 GFLOP;
 // one prompt of 65536 (D 128, 64 tokens, 40 heads over 8) 119 us for 2 * 134 MB and 2 * 43 GFLOP, 720 TFLOP/s.  The first
@@ -25,6 +25,11 @@ namespace psi {
 // a launch (at 104: 13.2 for 15.7 us in all, at 1460: 59 for 62, at 6656: 10.9 for 13.3); at 10240 the two come out even,
 // and at 30016 (55 us in all) repeating the join in every workgroup costs 4 us.
 constexpr uint64_t kFusedJoins = 8192;
+
+// Blocks of columns from which the waves of a short row share them: 64 tokens, 40 heads over 8, of one prompt of 1500
+// take 25 us for 34, 70 tokens, 12 heads over 2, of four of 413-826 35 us for 45; with 12 or 13 blocks sharing changes
+// little (14 prompts of 100: 28 us for 29, two of 550: 26 for 25).
+constexpr uint32_t kShareBlocks = 16;
 
 template <int kCtrl>
 __device__ __forceinline__ float dpp_of(float x) {
@@ -68,6 +73,7 @@ __global__ __launch_bounds__(64 * kWaves, kWaves / 4) void observe_kernel(Observ
     __shared__ __attribute__((aligned(16))) uint4 q_lds[kMaxBlocks * kSteps * 64];
     __shared__ int last_lds[kColumns];                                  // last key of the row that a column sees
     __shared__ float lse_lds[kSum ? kColumns : 1];
+    __shared__ float part_lds[kSum && kMaxBlocks >= kShareBlocks ? kWaves * kKeys : 1];  // sums over a part of the columns
     __shared__ float2 state_lds[kSum ? 1 : kWaves][kSum ? 1 : kColumns];  // maximum and sum so far
 
     const uint32_t row = blockIdx.x / a.v.hkv, kv_head = blockIdx.x % a.v.hkv;
@@ -83,6 +89,13 @@ __global__ __launch_bounds__(64 * kWaves, kWaves / 4) void observe_kernel(Observ
     for (uint32_t c0 = 0; c0 < columns; c0 += kColumns) {
         const uint32_t count = min(columns - c0, kColumns), blocks = (count + 16 * kBlocks - 1) / (16 * kBlocks) * kBlocks;
         const uint32_t key_end = min(r.end, r.position + (c0 + count - 1) / a.group + 1);  // what the last column sees
+        // Short rows of many columns: the waves that have no keys of their own share the columns of the others' keys.
+        const uint32_t length = key_end > r.begin ? key_end - r.begin : 0, key_groups = max((length + kKeys - 1) / kKeys, 1u);
+        const bool share = kMaxBlocks >= kShareBlocks && blocks >= kShareBlocks && key_groups * 2 <= kWaves;
+        const uint32_t parts = share ? min(kWaves / key_groups, blocks / kBlocks) : 1;
+        const uint32_t part = share ? wave / key_groups : 0, key_group = share ? wave % key_groups : wave;
+        const uint32_t part_blocks = (blocks / kBlocks + parts - 1) / parts * kBlocks;
+        const uint32_t block_begin = part * part_blocks, block_end = min(blocks, block_begin + part_blocks);
         // The page IDs of a wave's turn are asked for a turn ahead.  Its lines are not: a second buffer of them costs the
         // registers of a wave in three, and the other waves of the SIMD fill the wait better (one prompt of 65536, 64
         // tokens: 78 and 60 us a pass with two buffers, 68 and 57 with one).
@@ -121,8 +134,8 @@ __global__ __launch_bounds__(64 * kWaves, kWaves / 4) void observe_kernel(Observ
         // The second pass walks the turns backwards: what the first pass read last may still be in the cache of the XCD
         // (27.3 for 28.8 us at 8 prompts of 1k-8k, the same at 65536).  Loads are ordinary ones for that reason: streaming
         // ones take 33 + 31 us for 30 + 27, and 67 + 58 for 62 + 52 at 65536.
-        const uint32_t first = r.begin + wave * kKeys;
-        uint32_t turns = first < key_end ? (key_end - first + kTurn - 1) / kTurn : 0;
+        const uint32_t first = r.begin + key_group * kKeys;
+        uint32_t turns = first < key_end && block_begin < block_end ? (key_end - first + kTurn - 1) / kTurn : 0;
         const uint32_t step = kSum ? 0 - kTurn : kTurn;
         uint32_t base = kSum ? first + (turns - 1) * kTurn : first;
         if (turns > 0) {
@@ -183,7 +196,7 @@ __global__ __launch_bounds__(64 * kWaves, kWaves / 4) void observe_kernel(Observ
 #pragma unroll
                     for (int i = 0; i < 16; ++i) sums[w][i] = 0.0f;
             }
-            for (uint32_t b0 = 0; b0 < blocks; b0 += kBlocks) {
+            for (uint32_t b0 = block_begin; b0 < block_end; b0 += kBlocks) {
                 // kBlocks blocks at a time: independent products and exponentials to fill each other's latencies
                 f32x4_t acc[kBlocks][kTiles];
 #pragma unroll
@@ -246,8 +259,11 @@ __global__ __launch_bounds__(64 * kWaves, kWaves / 4) void observe_kernel(Observ
                 for (int w = 0; w < kWords; ++w) {
                     const float sum = row_sums(sums[w], lane);
                     const uint32_t tile = lane_row / 4, at = tile * 16 + lane_quarter * 4 + lane_row % 4, p = base + w * 64 + at;
-                    if (w * 4 + tile < kTiles && p < key_end && !(k.missing[w] >> at & 1))
+                    if (share) {
+                        if (w * 4 + tile < kTiles) part_lds[wave * kKeys + w * 64 + at] = sum;
+                    } else if (w * 4 + tile < kTiles && p < key_end && !(k.missing[w] >> at & 1)) {
                         add_weight(a, r, table, kv_head, p, sum, c0 == 0);
+                    }
                 }
             }
             if (turns > 1) {
@@ -269,6 +285,17 @@ __global__ __launch_bounds__(64 * kWaves, kWaves / 4) void observe_kernel(Observ
                 a.stats[stat_index(a, row, kv_head, c0 + i)] = make_float2(m, s);
             }
         } else {
+            if (share) {
+                // wave part * key_groups + g has its columns' sums for the keys of group g
+                lds_barrier();
+                const uint32_t summed = (blocks + part_blocks - 1) / part_blocks;
+                for (uint32_t i = tid; i < length; i += kThreads) {
+                    float sum = 0.0f;
+                    for (uint32_t q = 0; q < summed; ++q) sum += part_lds[q * key_groups * kKeys + i];
+                    if (page_of(a.v, table, r.begin + i, a.v.num_pages) != kNoPage)
+                        add_weight(a, r, table, kv_head, r.begin + i, sum, c0 == 0);
+                }
+            }
             // positions of the row that no column of the first columns sees still get their turn's base
             if (c0 == 0)
                 for (uint32_t p = max(key_end, r.begin) + tid; p < r.end; p += kThreads)

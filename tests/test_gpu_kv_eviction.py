@@ -263,6 +263,35 @@ def test_observation_leaves_out_pages_beyond_the_arena(psi, device):
     _assert_weights(weights.cpu().numpy()[mine], exp[mine], bound)
 
 
+@pytest.mark.parametrize("hq,hkv,d", [(40, 8, 128), (16, 2, 256)])
+def test_observation_of_many_columns_over_few_keys(psi, device, hq, hkv, d):
+    """Rows whose waves share the columns; a page beyond the arena in one prompt leaves its positions as they were and
+    the other prompt untouched."""
+    wl = importlib_workloads(psi)
+    w = wl.make_workload(28, [200, 330], hq, hkv, d, psi.Dtype.Bfloat16, 16, q_lens=[61, 64], **LAYERS)
+    acc = _weights(w)
+    exp, bound = attention_weights(w, w.pages, [150, 0], 0.5, acc)
+    got = _observe(psi, device, w, acc, [150, 0], 0.5).cpu().numpy()
+    for r in range(2):
+        p = np.arange(int(w.context_lens[r]))
+        at = (page_rows(w, r)[p // 16], slice(None), p % 16)
+        _assert_weights(got[at], exp[at], bound, f"prompt {r}")
+    rows, lay = page_rows(w, 0), w.layout
+    w.page_ids = w.page_ids.copy()
+    w.page_ids[(int(w.req_slots[0]) * lay.num_gqa_layers + w.layer) * lay.num_blocks + 2] = w.num_pages + 7
+    got = _observe(psi, device, w, acc, [150, 0], 0.5)
+    assert device.take_device_error() == psi._lib.DEVICE_ERR_CACHE_RANGE
+    got, mine = got.cpu().numpy(), page_rows(w, 1)[:-(-330 // 16)]
+    p = np.arange(330)
+    _assert_weights(got[mine[p // 16], :, p % 16], exp[mine[p // 16], :, p % 16], bound, "the other prompt")
+    assert np.array_equal(got[rows[2]], acc[rows[2]])
+    p = np.array([q for q in range(200) if q // 16 != 2])
+    mine = got[rows[p // 16], :, p % 16]
+    base = np.where(p < 150, 0.5, 0.0)[:, None] * acc[rows[p // 16], :, p % 16]
+    # (weights of the keys that are left sum to one per query)
+    assert np.abs((mine - base).sum(axis=0) / (61 * hq // hkv) - 1.0).max() <= 2.0 ** -24 * (4 * 200 + 61 * hq // hkv + 64)
+
+
 def test_observation_refusals(psi, device):
     import torch
 
