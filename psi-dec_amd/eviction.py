@@ -167,9 +167,18 @@ class GQAKVEvictionKernels:
                       else None)
         return GQAKVEvictionPlan(_upload(self.device, requests), len(rs), most.value, kept, buffer)
 
+    def _check_plan(self, plan: GQAKVEvictionPlan):
+        """A plan has room for what its own kernels keep: another budget or head count would leave it."""
+        wanted = (plan.num_reqs, self.config.num_kv_heads, self.budget)
+        if tuple(plan.kept.shape) != wanted or plan.kept.device != self.device.torch_device:
+            raise ValueError(f"plan: one prepared by kernels of this budget, head count and device is wanted; it keeps "
+                             f"{tuple(plan.kept.shape)} positions on {plan.kept.device}, these kernels {wanted}")
+
     def invoke_select(self, plan: GQAKVEvictionPlan, page_weights, page_ids, page_table_index: int):
         """The positions to keep, int32 [requests][KV heads][budget], ascending and padded with -1 (the 32-bit
-        sentinel); `plan.kept`, which the plan's next selection writes again."""
+        sentinel); `plan.kept`, which the plan's next selection writes again.  `plan` is one of these kernels' own, or of
+        others with the same budget, head count and page table layout."""
+        self._check_plan(plan)
         _check_page_weights(page_weights, self.device)
         L.check(self.device.lib.psi_hip_kv_select_kept(
             self.device.ctx, ctypes.byref(self._cfg), ctypes.byref(self._layout), _ptr(page_weights),
@@ -181,6 +190,7 @@ class GQAKVEvictionKernels:
         """Moves the kept lines of `kv_pages` and their accumulators (`page_weights` may be None) to the front."""
         import torch
 
+        self._check_plan(plan)
         if page_weights is not None:
             _check_page_weights(page_weights, self.device)
         if (kept.dtype != torch.int32 or not kept.is_contiguous() or kept.numel() != plan.kept.numel() or
