@@ -891,9 +891,10 @@ int psi_hip_kv_evict_plan(const psi_hip_gqa_config* cfg, const psi_hip_page_tabl
 int psi_hip_kv_select_scratch_bytes(const psi_hip_gqa_config* cfg, uint32_t num_reqs, uint32_t max_cached_tokens,
                                     uint64_t* out_bytes);
 
-/* kept: device u32[num_reqs][num_kv_heads][budget] with this call's budget (a buffer of a smaller one is written past its
- * end), the positions to keep in ascending order, padded with PSI_HIP_SENTINEL: all of a request of up to `budget` tokens; of a longer one the first num_first, the last num_recent
- * (together at most budget) and the heaviest of the others, of equal weights the lower position.  NaN counts as -inf.
+/* kept: device u32[num_reqs][num_kv_heads][budget] with this call's budget (a buffer of a smaller one is written past
+ * its end), the positions to keep in ascending order, padded with PSI_HIP_SENTINEL: all of a request of up to `budget`
+ * tokens; of a longer one the first num_first, the last num_recent (together at most budget) and the heaviest of the
+ * others, of equal weights the lower position.  NaN counts as -inf.
  * max_cached_tokens: the plan's.  scratch: device, 16-byte aligned, may be null when it needs no bytes.  Not while
  * device-side counts are bound. */
 int psi_hip_kv_select_kept(psi_hip_ctx* ctx, const psi_hip_gqa_config* cfg, const psi_hip_page_table_layout* layout,
@@ -903,11 +904,10 @@ int psi_hip_kv_select_kept(psi_hip_ctx* ctx, const psi_hip_gqa_config* cfg, cons
                            uint64_t scratch_bytes, uint32_t gqa_layer_index);
 
 /* Moves the K and V lines, and the accumulators unless page_weights is null, of position kept[i] to position i, in
- * place, for every request of more than `budget` tokens.  kept has the budget and requests of the selection that wrote it.
- * The kept positions of a (request, head) ascend, as the
- * selection writes them (in another order, the lines at its front are some of its cached lines); an entry that lies
- * outside the cached tokens or below its own index moves nothing.  Positions from `budget` on keep their bytes.  Up to
- * five launches for few long requests, otherwise one.  Not while device-side counts are bound. */
+ * place, for every request of more than `budget` tokens.  kept has the budget and requests of the selection that wrote
+ * it.  The kept positions of a (request, head) ascend, as the selection writes them (in another order, the lines at its
+ * front are some of its cached lines); an entry that lies outside the cached tokens or below its own index moves nothing.
+ * Positions from `budget` on keep their bytes.  Up to five launches for few long requests, otherwise one.  Not while device-side counts are bound. */
 int psi_hip_kv_compact(psi_hip_ctx* ctx, const psi_hip_gqa_config* cfg, const psi_hip_page_table_layout* layout,
                        void* kv_pages, uint64_t kv_pages_bytes, float* page_weights, uint64_t page_weights_bytes,
                        const uint32_t* page_ids, const uint32_t* requests, uint32_t num_reqs,

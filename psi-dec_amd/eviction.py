@@ -17,8 +17,8 @@ from typing import Optional, Sequence
 import numpy as np
 
 from . import _lib as L
-from .gqa import (Device, Dtype, GQAPageTableLayout, _cfg_struct, _check_page_weights, _nbytes, _ptr,
-                  _tokens_per_page)
+from .gqa import (Device, Dtype, GQAPageTableLayout, _cfg_struct, _check_page_weights, _is_stored, _nbytes,
+                  _ptr, _tokens_per_page)
 
 
 @dataclass(frozen=True)
@@ -112,10 +112,14 @@ class GQAKVObserveKernels:
                decay: float = 1.0):
         """Adds the windows' weights to `page_weights`; `q`: [query tokens][Q heads][head_dim], rotated."""
         _check_page_weights(page_weights, self.device)
-        if (q.numel() < plan.num_q_tokens * self.config.num_q_heads * self.config.head_dim or not q.is_contiguous() or
-                q.element_size() != self.config.dtype.item_size() or q.device != self.device.torch_device):
+        if (q.numel() < plan.num_q_tokens * self.config.num_q_heads * self.config.head_dim or
+                q.element_size() != self.config.dtype.item_size() or not _is_stored(q, self.config.dtype, self.device)):
             raise ValueError("q: contiguous rows of the cache's type on the kernels' device are wanted, one for every "
                              "planned query token")
+        if not _is_stored(kv_pages, self.config.dtype, self.device):
+            raise ValueError("kv_pages: a contiguous arena of the configured type on the kernels' device is wanted")
+        if plan.scratch.device != self.device.torch_device:
+            raise ValueError("plan: one prepared on the kernels' device is wanted")
         L.check(self.device.lib.psi_hip_kv_observe_weights(
             self.device.ctx, ctypes.byref(self._cfg), ctypes.byref(self._layout), _ptr(q), plan.num_q_tokens,
             _ptr(kv_pages), _nbytes(kv_pages), _ptr(page_ids), _ptr(plan.windows), plan.num_windows, plan.max_window,
@@ -196,6 +200,8 @@ class GQAKVEvictionKernels:
         if (kept.dtype != torch.int32 or not kept.is_contiguous() or kept.numel() != plan.kept.numel() or
                 kept.device != self.device.torch_device):
             raise ValueError("kept: the contiguous int32 [requests][KV heads][budget] of a selection is wanted")
+        if not _is_stored(kv_pages, self.config.dtype, self.device):
+            raise ValueError("kv_pages: a contiguous arena of the configured type on the kernels' device is wanted")
         L.check(self.device.lib.psi_hip_kv_compact(
             self.device.ctx, ctypes.byref(self._cfg), ctypes.byref(self._layout), _ptr(kv_pages), _nbytes(kv_pages),
             _ptr(page_weights), _nbytes(page_weights), _ptr(page_ids), _ptr(plan.requests), plan.num_reqs,

@@ -1034,6 +1034,12 @@ def _check_page_weights(weights, device: Device):
         raise ValueError("page_weights: a contiguous float32 tensor on the kernels' device is wanted")
 
 
+def _is_stored(t, dtype: Dtype, device: Device) -> bool:
+    """Contiguous storage of `dtype` on the kernels' device; integers are taken as its bytes."""
+    of_type = t.dtype == dtype.torch() or not (t.is_floating_point() or t.is_complex())
+    return of_type and t.is_contiguous() and t.device == device.torch_device
+
+
 @dataclass
 class GQAKVWeights:
     """psi_hip_kv_weights: what a decode step adds its attention weights to (`page_weights` of eviction.py) and the
@@ -1044,6 +1050,8 @@ class GQAKVWeights:
 
     def struct(self, device: Device):
         _check_page_weights(self.page_weights, device)
+        if self.logits.buffer.device != device.torch_device:
+            raise ValueError("logits: room on the kernels' device is wanted")
         return L.KVWeightsStruct(self.page_weights.data_ptr(), _nbytes(self.page_weights), self.logits.buffer.data_ptr(),
                                  self.logits.bytes, self.logits.max_context_tokens, self.decay)
 
