@@ -887,7 +887,8 @@ int psi_hip_kv_evict_plan(const psi_hip_gqa_config* cfg, const psi_hip_page_tabl
                           const uint32_t* req_slots, const uint32_t* num_cached, uint32_t num_reqs, uint32_t* requests,
                           uint32_t* out_max_cached);
 
-/* Bytes of a selection's scratch (0 while no request holds more than 16384 tokens). */
+/* Bytes of a selection's scratch (0 while no request holds more than 16384 tokens).  Scratch of a capacity serves every
+ * selection of no more requests and no longer ones. */
 int psi_hip_kv_select_scratch_bytes(const psi_hip_gqa_config* cfg, uint32_t num_reqs, uint32_t max_cached_tokens,
                                     uint64_t* out_bytes);
 

@@ -6,6 +6,8 @@
 // LDS), the positions by ballots and prefix counts: no sort, and the same answer on every run.
 #include "kv_eviction.h"
 
+#include <algorithm>
+
 namespace psi {
 
 struct SelectArgs {
@@ -255,7 +257,14 @@ inline uint64_t select_chunks(uint32_t max_cached, int quads) {
 // Chunks of 4096 while those of 8192 would leave half of the compute units without one (4 requests of 131072 on 2 heads: 28
 // us for 30; 6 of up to 38290 on 4 heads: 25 for 29), which costs a chunk twice the counters to add up (40 requests of
 // 30000 on 8 heads: 128 us for 100).
-inline int chunk_quads(uint64_t rows, uint32_t max_cached) { return rows * select_chunks(max_cached, 2) <= 128 ? 1 : 2; }
+constexpr uint64_t kFewChunks = 128;
+inline int chunk_quads(uint64_t rows, uint32_t max_cached) { return rows * select_chunks(max_cached, 2) <= kFewChunks ? 1 : 2; }
+// Chunks that the scratch of a capacity holds: those of every selection of fewer rows or shorter requests too, though a
+// launch of small chunks can have more of them than a larger one of large chunks.
+inline uint64_t scratch_chunks(uint64_t rows, uint32_t max_cached) {
+    static_assert(chunk_keys(2) == 2 * chunk_keys(1), "a large chunk makes at most two small ones");
+    return std::max(rows * select_chunks(max_cached, 2), std::min(rows * select_chunks(max_cached, 1), 2 * kFewChunks));
+}
 
 // kPass 0 .. 2: counts digit kPass; kPass 3: writes the positions.
 template <int kPass, int kChunkQuads>
@@ -347,8 +356,9 @@ extern "C" int psi_hip_kv_select_scratch_bytes(const psi_hip_gqa_config* cfg, ui
     PSI_REQUIRE(out_bytes != nullptr, "out pointer must not be null");
     PSI_REQUIRE(num_reqs > 0, "a selection needs requests");
     const uint64_t rows = (uint64_t)num_reqs * g.hkv;
-    const uint64_t chunks = rows * select_chunks(max_cached_tokens, chunk_quads(rows, max_cached_tokens));
-    *out_bytes = max_cached_tokens <= kRowPositions ? 0 : chunks * (kDigits * kBins * 2 + sizeof(ChunkState));
+    *out_bytes = max_cached_tokens <= kRowPositions
+                     ? 0
+                     : scratch_chunks(rows, max_cached_tokens) * (kDigits * kBins * 2 + sizeof(ChunkState));
     return PSI_HIP_OK;
 }
 
