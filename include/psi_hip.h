@@ -140,8 +140,10 @@ int psi_hip_ctx_set_flag(psi_hip_ctx* ctx, uint32_t flag, uint32_t value);
  *                 more than 48 query columns, which that entry point hands to the same kernel: for those, set
  *                 PSI_HIP_FLAG_FORCE_GENERIC for the step (the shape-generic kernels multiply in f32);
  *   CACHE_RANGE   an operator of the section "cache eviction" met a request slot, position or page ID outside the
- *                 bounds it was given (the page table, the arena, the accumulators, max_context_tokens, a table of
- *                 kept positions that does not ascend): what it names was left out and stays as it was.
+ *                 bounds it was given (the page table, the arena, the accumulators, max_context_tokens) or a kept
+ *                 position below its own index: what it names was left out and stays as it was.  (The decode attention
+ *                 that accumulates checks what it accumulates; K and V it reads and appends as every decode step does,
+ *                 through slots and page IDs that it trusts.)
  * psi_hip_sync returns PSI_HIP_ERR_RUNTIME while a bit is set; psi_hip_ctx_take_device_error
  * synchronises the context's stream, returns the bits and clears them. */
 #define PSI_HIP_DEVICE_ERR_WAIT_GAVE_UP 1u
@@ -813,7 +815,9 @@ int psi_hip_gqa_replay_cache_stats(const psi_hip_gqa_replay_cache* cache, uint32
  * Accumulators: page_weights, device f32 [page][num_kv_heads][tokens_per_page], found through the same page IDs as K
  * and V (every layer's pages are its own, so one array serves all layers).  A step starts the accumulators of the
  * tokens it appends from zero, so a page taken from the allocator needs no clearing.  A page belongs to one request;
- * page IDs beyond the arena or the accumulators are left out (PSI_HIP_DEVICE_ERR_CACHE_RANGE).
+ * accumulators of page IDs beyond the arena or the accumulators are left out (PSI_HIP_DEVICE_ERR_CACHE_RANGE), and so are
+ * the K and V lines of such pages in observe_weights and compact.  attend_weights reads and appends K and V as the plain
+ * decode map does: request slots and page IDs have to be valid there.
  * Weights, normalisers and sums are f32 whatever the cache's type.  Nothing is added atomically: the same call gives
  * the same bits on every run.  These entry points allocate nothing and can be captured into a graph; two launches of
  * one scratch, logits or kept buffer must follow one another. */

@@ -4,6 +4,8 @@
 //     w[h][p] = sum over the step's tokens t of the request, p <= position(t), and over the query heads g of KV head h of
 //               exp2(logit[t][g][p] - max[t][g]) / sum[t][g],
 // and adds them to the accumulators:  acc = (p appended before this step ? decay * acc : 0) + w.
+#include <algorithm>
+
 #include "kv_eviction.h"
 #include "split_kv_reduce_kernel.h"
 
@@ -70,6 +72,10 @@ __device__ __forceinline__ void accumulate_row(const WeightsArgs& a, uint32_t sp
     const uint32_t slot = a.req_slots[token], slot_before = a.req_slots[before], slot_after = a.req_slots[after];
     const uint32_t own = a.flat_token_indices[token], p0 = a.cu_kv_splits[token], p1 = a.cu_kv_splits[token + 1];
     if (after != token && slot_after == slot) return;
+    if (slot >= a.v.num_slots) {
+        report_cache_range(a.status);
+        return;
+    }
     uint32_t first = token, held = own;
     if (before != token && slot_before == slot) {
         for (first = before; first > 0 && a.req_slots[first - 1] == slot;) --first;
@@ -258,6 +264,7 @@ extern "C" int psi_hip_split_kv_single_q_attend_weights(
     rc = make_cache_view(g, layout, page_ids, gqa_layer_index, kv_pages_bytes, weights->page_weights_bytes, &a.v);
     if (rc != PSI_HIP_OK) return rc;
     PSI_REQUIRE((uint64_t)num_total_kv_splits * g.hkv <= 0x7fffffffull, "too many KV splits");
+    a.v.num_weight_pages = std::min(a.v.num_weight_pages, a.v.num_pages);  // no page beyond the arena either
 
     DeviceGuard guard(ctx->device);
     float* logits = static_cast<float*>(weights->logits);
