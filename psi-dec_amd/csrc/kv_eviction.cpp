@@ -156,7 +156,7 @@ extern "C" int psi_hip_kv_observe_plan(const psi_hip_gqa_config* cfg, const psi_
     PSI_REQUIRE(n <= UINT32_MAX, "observation plan: too many rows");
     *out_num_rows = (uint32_t)n;
     *out_max_window = max_window;
-    *out_scratch_bytes = (n * max_window * 2 + cu_tokens[num_reqs]) * g.hq * 4;
+    *out_scratch_bytes = (n * max_window + cu_tokens[num_reqs]) * g.hq * 8;
     return PSI_HIP_OK;
 }
 

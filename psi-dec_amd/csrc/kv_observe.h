@@ -1,7 +1,7 @@
 // Shared declarations of the observation kernels: attention weights of a window of query tokens over its request's
 // cached keys, summed per key and KV head and added to the accumulators, without the attention's output:
 //     w[h][p] = sum over the window's tokens t with p <= position(t), and over the query heads g of KV head h, of
-//               exp2(l[t][g][p] - lse[t][g]),   l = scale * log2(e) * q . k,   lse = log2 sum_p exp2(l).
+//               exp2(l[t][g][p] - m[t][g]) / s[t][g],   l = scale * log2(e) * q . k,   m = max_p l,   s = sum_p exp2(l - m).
 // The normaliser must be known before a weight is, so the keys are walked twice: a pass for the maximum and sum of every
 // (row, column), and a pass that joins those of a window's rows, recomputes the logits and sums the weights.  A row is a
 // range of keys of one window (psi_hip_kv_observe_plan), a column a (token of the window, query head of the KV head).  A
@@ -23,7 +23,7 @@ struct ObserveArgs {
     uint32_t hq, group;
     float scale_log2, decay;
     float2* stats;  // [row][kv head][token in window][head of the group]: maximum (log2 domain) and sum
-    float* lse;     // [query row][q head]; null in the second pass: joined there
+    float2* norm;   // [query row][q head]: maximum and reciprocal sum; null in the second pass: joined there
     float* page_weights;
     uint32_t* status;
 };
@@ -63,8 +63,11 @@ __device__ __forceinline__ void join_states(float2 part, float* m, float* s) {
     *s = *s * exp2f(*m - next) + part.y * exp2f(part.x - next);
     *m = next;
 }
-// +inf where no key contributes, so that the column's weights are zero.
-__device__ __forceinline__ float lse_of_state(float m, float s) { return s == 0.0f ? INFINITY : m + log2f(s); }
+// What a weight is made of: exp2(l - x) * y.  +inf and 0 where no key contributes, so that the column's weights are zero.
+// (The sum stays out of the exponent: half an ulp of its log2 would be an error of all the column's weights alike.)
+__device__ __forceinline__ float2 norm_of_state(float m, float s) {
+    return s == 0.0f ? make_float2(INFINITY, 0.0f) : make_float2(m, 1.0f / s);
+}
 // The states of one column over rows first, first + step, ... before row_end.
 __device__ __forceinline__ void join_rows(const ObserveArgs& a, uint32_t first, uint32_t row_end, uint32_t step,
                                           uint32_t kv_head, uint32_t column, float* m, float* s) {
@@ -80,7 +83,7 @@ __device__ __forceinline__ void join_rows(const ObserveArgs& a, uint32_t first, 
     }
 }
 // The same by `parts` adjacent lanes (a power of two), each of which gets the normaliser of the column.
-__device__ __forceinline__ float join_column(const ObserveArgs& a, const ObserveRow& r, uint32_t kv_head, uint32_t column,
+__device__ __forceinline__ float2 join_column(const ObserveArgs& a, const ObserveRow& r, uint32_t kv_head, uint32_t column,
                                              uint32_t part, uint32_t parts) {
     float m = kEmptyMax, s = 0.0f;
     join_rows(a, r.row_begin + part, r.row_end, parts, kv_head, column, &m, &s);
@@ -88,7 +91,7 @@ __device__ __forceinline__ float join_column(const ObserveArgs& a, const Observe
         const float2 other = make_float2(__shfl_xor(m, off, 64), __shfl_xor(s, off, 64));
         join_states(other, &m, &s);
     }
-    return lse_of_state(m, s);
+    return norm_of_state(m, s);
 }
 
 // First weights of a position in this call: on top of what counts already.  Later ones: on top of the first.
@@ -103,7 +106,7 @@ __device__ __forceinline__ void add_weight(const ObserveArgs& a, const ObserveRo
     *acc = (!first ? *acc : p < r.held ? a.decay * *acc : 0.0f) + sum;
 }
 
-// The normalisers of all query rows and heads into a.lse, between the two passes.
+// The normalisers of all query rows and heads into a.norm, between the two passes.
 void launch_observe_join(psi_hip_ctx* ctx, const ObserveArgs& a);
 
 // Matrix-core kernels (kv_observe_kernel.h), one translation unit per element type; head_dim 128 or 256.

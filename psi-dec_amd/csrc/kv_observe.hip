@@ -62,7 +62,7 @@ __global__ __launch_bounds__(kJoinItems * kJoinParts) void observe_join(ObserveA
     __syncthreads();
     if (part != 0 || !live) return;
     for (uint32_t i = 1; i < kJoinParts; ++i) join_states(parts[i][threadIdx.x], &m, &s);
-    a.lse[(uint64_t)(q_begin + column / a.group) * a.hq + kv_head * a.group + column % a.group] = lse_of_state(m, s);
+    a.norm[(uint64_t)(q_begin + column / a.group) * a.hq + kv_head * a.group + column % a.group] = norm_of_state(m, s);
 }
 
 void launch_observe_join(psi_hip_ctx* ctx, const ObserveArgs& a) {
@@ -87,7 +87,8 @@ __global__ __launch_bounds__(256) void observe_sum_generic(ObserveArgs a) {
             float sum = 0.0f;
             for (uint32_t g = 0; g < a.group; ++g) {
                 const uint64_t at = (uint64_t)(r.q_begin + t) * a.hq + kv_head * a.group + g;
-                sum += exp2f(dot_line<Tag>(a, at * a.v.d, k_off) * a.scale_log2 - a.lse[at]);
+                const float2 norm = a.norm[at];
+                sum += exp2f(dot_line<Tag>(a, at * a.v.d, k_off) * a.scale_log2 - norm.x) * norm.y;
             }
             total += sum;
         }
@@ -121,7 +122,7 @@ extern "C" int psi_hip_kv_observe_weights(psi_hip_ctx* ctx, const psi_hip_gqa_co
     rc = make_cache_view(g, layout, page_ids, gqa_layer_index, kv_pages_bytes, page_weights_bytes, &a.v);
     if (rc != PSI_HIP_OK) return rc;
     const uint64_t stats = (uint64_t)num_rows * max_window * g.hq;
-    const uint64_t needed = (2 * stats + (uint64_t)num_q_tokens * g.hq) * 4;
+    const uint64_t needed = (stats + (uint64_t)num_q_tokens * g.hq) * sizeof(float2);
     PSI_REQUIRE(scratch_bytes >= needed, "observation scratch too small: %llu < %llu", (unsigned long long)scratch_bytes,
                 (unsigned long long)needed);
     PSI_REQUIRE(reinterpret_cast<uintptr_t>(scratch) % 8 == 0, "the observation scratch must be 8-byte aligned");
@@ -141,7 +142,7 @@ extern "C" int psi_hip_kv_observe_weights(psi_hip_ctx* ctx, const psi_hip_gqa_co
     a.scale_log2 = g.scale * kLog2eObserve;
     a.decay = decay;
     a.stats = static_cast<float2*>(scratch);
-    a.lse = reinterpret_cast<float*>(a.stats + stats);
+    a.norm = a.stats + stats;
     a.page_weights = page_weights;
     a.status = ctx->status_device;
 

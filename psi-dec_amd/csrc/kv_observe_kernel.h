@@ -72,7 +72,7 @@ __global__ __launch_bounds__(64 * kWaves, kWaves / 4) void observe_kernel(Observ
     constexpr uint32_t kKeys = 16 * kTiles, kTurn = kWaves * kKeys;  // keys of a wave's turn, of all waves'
     __shared__ __attribute__((aligned(16))) uint4 q_lds[kMaxBlocks * kSteps * 64];
     __shared__ int last_lds[kColumns];                                  // last key of the row that a column sees
-    __shared__ float lse_lds[kSum ? kColumns : 1];
+    __shared__ float2 norm_lds[kSum ? kColumns : 1];
     __shared__ float part_lds[kSum && kMaxBlocks >= kShareBlocks ? kWaves * kKeys : 1];  // sums over a part of the columns
     __shared__ float2 state_lds[kSum ? 1 : kWaves][kSum ? 1 : kColumns];  // maximum and sum so far
 
@@ -166,19 +166,20 @@ __global__ __launch_bounds__(64 * kWaves, kWaves / 4) void observe_kernel(Observ
         for (uint32_t i = tid; i < blocks * 16; i += kThreads) {
             const uint32_t c = c0 + i;
             last_lds[i] = c < columns ? (int)min(r.position + c / a.group, key_end - 1) : -1;
-            if (kSum && (a.lse != nullptr || c >= columns))
-                lse_lds[i] = c >= columns ? INFINITY
-                                          : a.lse[(uint64_t)(r.q_begin + c / a.group) * a.hq + kv_head * a.group + c % a.group];
+            if (kSum && (a.norm != nullptr || c >= columns))
+                norm_lds[i] = c >= columns
+                                  ? make_float2(INFINITY, 0.0f)
+                                  : a.norm[(uint64_t)(r.q_begin + c / a.group) * a.hq + kv_head * a.group + c % a.group];
         }
-        if (kSum && a.lse == nullptr) {
+        if (kSum && a.norm == nullptr) {
             // a column's rows are shared out among the lanes that its neighbours leave (8 tokens of 13234, 208 rows: 10.9
             // us for 19.8 with a lane a column)
             const uint32_t rows = r.row_end - min(r.row_begin, r.row_end);
             uint32_t parts = 1;
             while (parts < 64 && 2 * parts * count <= kThreads && 8 * parts < rows) parts *= 2;
             for (uint32_t i = tid; i < count * parts; i += kThreads) {
-                const float lse = join_column(a, r, kv_head, c0 + i / parts, i % parts, parts);
-                if (i % parts == 0) lse_lds[i / parts] = lse;
+                const float2 norm = join_column(a, r, kv_head, c0 + i / parts, i % parts, parts);
+                if (i % parts == 0) norm_lds[i / parts] = norm;
             }
         }
         if constexpr (!kSum)
@@ -244,12 +245,14 @@ __global__ __launch_bounds__(64 * kWaves, kWaves / 4) void observe_kernel(Observ
                         sum = fmaf(old.y, __builtin_amdgcn_exp2f(old.x - next), quarter_wave_sum(sum));
                         if (lane < 16) state_lds[wave][column] = make_float2(next, sum);
                     } else {
-                        const float lse = lse_lds[column];
+                        const float2 norm = norm_lds[column];
 #pragma unroll
                         for (int t = 0; t < kTiles; ++t)
 #pragma unroll
-                            for (int e = 0; e < 4; ++e)
-                                sums[t / 4][t % 4 * 4 + e] += __builtin_amdgcn_exp2f(fmaf(acc[h][t][e], a.scale_log2, -lse));
+                            for (int e = 0; e < 4; ++e) {
+                                float& sum = sums[t / 4][t % 4 * 4 + e];
+                                sum = fmaf(__builtin_amdgcn_exp2f(fmaf(acc[h][t][e], a.scale_log2, -norm.x)), norm.y, sum);
+                            }
                     }
                 }
             }
@@ -315,10 +318,10 @@ inline void launch_observe_blocks(psi_hip_ctx* ctx, const ObserveArgs& a) {
     const dim3 grid(a.num_rows * a.v.hkv);
     ObserveArgs fused = a;
     const uint64_t joins = (uint64_t)a.num_rows / a.num_windows * a.max_window * a.group;
-    if (joins <= kFusedJoins) fused.lse = nullptr;
+    if (joins <= kFusedJoins) fused.norm = nullptr;
     hipLaunchKernelGGL((observe_kernel<Tag, D, Stats::kTiles, Stats::kBlocks, kMaxBlocks, Stats::kWaves, false>), grid,
                        dim3(64 * Stats::kWaves), 0, ctx->stream, a);
-    if (fused.lse != nullptr) launch_observe_join(ctx, a);
+    if (fused.norm != nullptr) launch_observe_join(ctx, a);
     hipLaunchKernelGGL((observe_kernel<Tag, D, Sum::kTiles, Sum::kBlocks, kMaxBlocks, Sum::kWaves, true>), grid,
                        dim3(64 * Sum::kWaves), 0, ctx->stream, fused);
 }

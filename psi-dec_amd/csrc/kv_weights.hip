@@ -30,12 +30,13 @@ struct WeightsArgs {
 };
 
 constexpr uint32_t kFinishThreads = 512, kFinishWaves = kFinishThreads / 64;
-constexpr uint32_t kLseEntries = 512;  // (token, head) normalisers held in LDS at a time
+constexpr uint32_t kNormEntries = 512;  // (token, head) normalisers held in LDS at a time
 constexpr uint32_t kFewEntries = 8;    // up to this many (a decode step's heads) a thread holds the logits of all
 
-// log2 of the sum of exponentials of one (token, head) over its partial states p0 .. p1, in every lane of the wave;
-// +inf where nothing contributes, so that the row's weights are zero.
-__device__ __forceinline__ float lse_of(const WeightsArgs& a, uint32_t p0, uint32_t p1, uint32_t head, uint32_t lane) {
+// Maximum and reciprocal sum of one (token, head) over its partial states p0 .. p1, in every lane of the wave; +inf and 0
+// where nothing contributes, so that the row's weights are zero.  The sum stays out of the exponent: half an ulp of its
+// log2 would be an error of all the row's weights alike.
+__device__ __forceinline__ float2 norm_of(const WeightsArgs& a, uint32_t p0, uint32_t p1, uint32_t head, uint32_t lane) {
     float m = -INFINITY, s = 0.0f;
     for (uint32_t p = p0 + lane; p < p1; p += 64) {
         const uint64_t r = (uint64_t)(a.row_index ? a.row_index[p] : p) * a.hq + head;
@@ -49,7 +50,7 @@ __device__ __forceinline__ float lse_of(const WeightsArgs& a, uint32_t p0, uint3
         if (next > -INFINITY) s = s * exp2f(m - next) + os * exp2f(om - next);
         m = next;
     }
-    return m > -INFINITY ? m + log2f(s) : INFINITY;
+    return m > -INFINITY ? make_float2(m, 1.0f / s) : make_float2(INFINITY, 0.0f);
 }
 
 // The accumulators of one (kv_split row, KV head), by a workgroup.  The rows of a request's last token of the step tile
@@ -60,7 +61,7 @@ __device__ __forceinline__ float lse_of(const WeightsArgs& a, uint32_t p0, uint3
 // round trip), so the first turn's logits and page IDs are asked for before the normalisers are.  With the combine beside
 // it: 11.4 us for 25 MB at 32 requests of 1k-8k (the combine alone takes 6), 13.0 us for 49 MB (3.8 TB/s) at four of
 // 131072; two to four workgroups a row repeat the chain and take longer (an earlier form: 22 us for 15).
-__device__ __forceinline__ void accumulate_row(const WeightsArgs& a, uint32_t split, uint32_t kv_head, float* lse) {
+__device__ __forceinline__ void accumulate_row(const WeightsArgs& a, uint32_t split, uint32_t kv_head, float2* norm) {
     const uint32_t num_tokens = active_count(a.replay_counts, kReplayTokens, a.num_active_tokens);
     const uint32_t num_splits = active_count(a.replay_counts, kReplaySplits, a.num_active_kv_splits);
     const uint32_t layer = active_layer(a.replay_counts, a.v.layer, a.v.num_layers);
@@ -133,8 +134,8 @@ __device__ __forceinline__ void accumulate_row(const WeightsArgs& a, uint32_t sp
         };
         if (start < end) fetch(start);
         if (wave < entries) {
-            const float x = lse_of(a, p0, p1, kv_head * a.group + wave, lane);
-            if (lane == 0) lse[wave] = x;
+            const float2 x = norm_of(a, p0, p1, kv_head * a.group + wave, lane);
+            if (lane == 0) norm[wave] = x;
         }
         __syncthreads();
         for (uint32_t p = start; p < end; p += kFinishThreads * 4) {
@@ -145,19 +146,20 @@ __device__ __forceinline__ void accumulate_row(const WeightsArgs& a, uint32_t sp
                 if (e >= entries) continue;
                 const float x[4] = {l[e].x, l[e].y, l[e].z, l[e].w};
 #pragma unroll
-                for (int i = 0; i < 4; ++i) sum[i] += p + i <= own ? __builtin_amdgcn_exp2f(x[i] - lse[e]) : 0.0f;
+                for (int i = 0; i < 4; ++i)
+                    sum[i] += p + i <= own ? __builtin_amdgcn_exp2f(x[i] - norm[e].x) * norm[e].y : 0.0f;
             }
             add(p, sum, page, old, true);
         }
         return;
     }
-    for (uint32_t base = 0; base < entries; base += kLseEntries) {
-        const uint32_t count = min(kLseEntries, entries - base);
+    for (uint32_t base = 0; base < entries; base += kNormEntries) {
+        const uint32_t count = min(kNormEntries, entries - base);
         if (base > 0) __syncthreads();
         for (uint32_t e = wave; e < count; e += kFinishWaves) {
             const uint32_t t = first + (base + e) / a.group;
-            const float x = lse_of(a, a.cu_kv_splits[t], a.cu_kv_splits[t + 1], kv_head * a.group + (base + e) % a.group, lane);
-            if (lane == 0) lse[e] = x;
+            const float2 x = norm_of(a, a.cu_kv_splits[t], a.cu_kv_splits[t + 1], kv_head * a.group + (base + e) % a.group, lane);
+            if (lane == 0) norm[e] = x;
         }
         __syncthreads();
         for (uint32_t p = start; p < end; p += kFinishThreads * 4) {
@@ -170,7 +172,8 @@ __device__ __forceinline__ void accumulate_row(const WeightsArgs& a, uint32_t sp
                     a.logits + logit_index(a.logits_stride, a.group, (uint64_t)(first + t) * a.v.hkv + kv_head, p, g));
                 const float x[4] = {l.x, l.y, l.z, l.w};
 #pragma unroll
-                for (int i = 0; i < 4; ++i) sum[i] += p + i <= last ? __builtin_amdgcn_exp2f(x[i] - lse[e]) : 0.0f;
+                for (int i = 0; i < 4; ++i)
+                    sum[i] += p + i <= last ? __builtin_amdgcn_exp2f(x[i] - norm[e].x) * norm[e].y : 0.0f;
                 if (++g == a.group) {
                     g = 0;
                     ++t;
@@ -188,12 +191,12 @@ template <typename Tag, int D>
 __global__ __launch_bounds__(kFinishThreads) void finish_kernel(WeightsArgs w, ReduceArgs r, uint32_t weight_groups,
                                                                 uint32_t wide) {
     __shared__ union {
-        float lse[kLseEntries];
+        float2 norm[kNormEntries];
         WideReduceLds<D> wide;
     } lds;
     static_assert(kWideWaves == kFinishWaves, "a wide row takes the whole workgroup");
     if (blockIdx.x < weight_groups) {
-        accumulate_row(w, blockIdx.x / w.v.hkv, blockIdx.x % w.v.hkv, lds.lse);
+        accumulate_row(w, blockIdx.x / w.v.hkv, blockIdx.x % w.v.hkv, lds.norm);
         return;
     }
     resolve_active(r);
@@ -211,8 +214,8 @@ __global__ __launch_bounds__(kFinishThreads) void finish_kernel(WeightsArgs w, R
 
 // The accumulators alone, next to the shape-generic combine.
 __global__ __launch_bounds__(kFinishThreads) void accumulate_kernel(WeightsArgs w) {
-    __shared__ float lse[kLseEntries];
-    accumulate_row(w, blockIdx.x / w.v.hkv, blockIdx.x % w.v.hkv, lse);
+    __shared__ float2 norm[kNormEntries];
+    accumulate_row(w, blockIdx.x / w.v.hkv, blockIdx.x % w.v.hkv, norm);
 }
 
 static uint64_t logits_stride(uint32_t max_context_tokens) { return ((uint64_t)max_context_tokens + 63) / 64 * 64; }
