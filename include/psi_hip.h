@@ -884,6 +884,16 @@ int psi_hip_kv_observe_weights(psi_hip_ctx* ctx, const psi_hip_gqa_config* cfg, 
                                uint32_t max_window, const uint32_t* rows, uint32_t num_rows, void* scratch,
                                uint64_t scratch_bytes, float* page_weights, uint64_t page_weights_bytes, float decay,
                                uint32_t gqa_layer_index);
+/* The same, told how many rows the window of most rows has (the largest windows[r][6] - windows[r][5] of the plan; 0: not
+ * known, the call above).  Results do not depend on it beyond rounding: it decides whether the windows' statistics are
+ * joined in a launch of their own, which a call that is not told assumes to pay unless no window can be long. */
+int psi_hip_kv_observe_weights_rows(psi_hip_ctx* ctx, const psi_hip_gqa_config* cfg,
+                                    const psi_hip_page_table_layout* layout, const void* q, uint32_t num_q_tokens,
+                                    const void* kv_pages, uint64_t kv_pages_bytes, const uint32_t* page_ids,
+                                    const uint32_t* windows, uint32_t num_windows, uint32_t max_window,
+                                    const uint32_t* rows, uint32_t num_rows, uint32_t max_window_rows, void* scratch,
+                                    uint64_t scratch_bytes, float* page_weights, uint64_t page_weights_bytes,
+                                    float decay, uint32_t gqa_layer_index);
 
 /* Host plan of an eviction: request r holds num_cached[r] tokens (0 is allowed).  A slot may be named once.  requests:
  * host u32[num_reqs][2], to be copied to the device for the two calls below; *out_max_cached: the longest. */

@@ -401,6 +401,9 @@ PROTOTYPES = {
     "psi_hip_kv_observe_weights": (
         c_int, [c_void_p, _CFG, _LAYOUT, c_void_p, c_uint32, c_void_p, c_uint64, c_void_p, c_void_p, c_uint32, c_uint32,
                 c_void_p, c_uint32, c_void_p, c_uint64, c_void_p, c_uint64, c_float, c_uint32]),
+    "psi_hip_kv_observe_weights_rows": (
+        c_int, [c_void_p, _CFG, _LAYOUT, c_void_p, c_uint32, c_void_p, c_uint64, c_void_p, c_void_p, c_uint32, c_uint32,
+                c_void_p, c_uint32, c_uint32, c_void_p, c_uint64, c_void_p, c_uint64, c_float, c_uint32]),
     "psi_hip_kv_evict_plan": (c_int, [_CFG, _LAYOUT, _U32P, _U32P, c_uint32, _U32P, _U32P]),
     "psi_hip_kv_select_scratch_bytes": (c_int, [_CFG, c_uint32, c_uint32, POINTER(c_uint64)]),
     "psi_hip_kv_select_kept": (

@@ -109,8 +109,9 @@ __device__ __forceinline__ void add_weight(const ObserveArgs& a, const ObserveRo
 // The normalisers of all query rows and heads into a.norm, between the two passes.
 void launch_observe_join(psi_hip_ctx* ctx, const ObserveArgs& a);
 
-// Matrix-core kernels (kv_observe_kernel.h), one translation unit per element type; head_dim 128 or 256.
-void launch_observe_bf16(psi_hip_ctx* ctx, const ObserveArgs& a);
-void launch_observe_f16(psi_hip_ctx* ctx, const ObserveArgs& a);
+// Matrix-core kernels (kv_observe_kernel.h), one translation unit per element type; head_dim 128 or 256.  window_rows: the
+// most rows that one window has.
+void launch_observe_bf16(psi_hip_ctx* ctx, const ObserveArgs& a, uint32_t window_rows);
+void launch_observe_f16(psi_hip_ctx* ctx, const ObserveArgs& a, uint32_t window_rows);
 
 }  // namespace psi

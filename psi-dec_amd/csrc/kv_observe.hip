@@ -107,6 +107,19 @@ extern "C" int psi_hip_kv_observe_weights(psi_hip_ctx* ctx, const psi_hip_gqa_co
                                           const uint32_t* rows, uint32_t num_rows, void* scratch, uint64_t scratch_bytes,
                                           float* page_weights, uint64_t page_weights_bytes, float decay,
                                           uint32_t gqa_layer_index) {
+    return psi_hip_kv_observe_weights_rows(ctx, cfg, layout, q, num_q_tokens, kv_pages, kv_pages_bytes, page_ids, windows,
+                                           num_windows, max_window, rows, num_rows, 0, scratch, scratch_bytes,
+                                           page_weights, page_weights_bytes, decay, gqa_layer_index);
+}
+
+extern "C" int psi_hip_kv_observe_weights_rows(psi_hip_ctx* ctx, const psi_hip_gqa_config* cfg,
+                                               const psi_hip_page_table_layout* layout, const void* q,
+                                               uint32_t num_q_tokens, const void* kv_pages, uint64_t kv_pages_bytes,
+                                               const uint32_t* page_ids, const uint32_t* windows, uint32_t num_windows,
+                                               uint32_t max_window, const uint32_t* rows, uint32_t num_rows,
+                                               uint32_t max_window_rows, void* scratch, uint64_t scratch_bytes,
+                                               float* page_weights, uint64_t page_weights_bytes, float decay,
+                                               uint32_t gqa_layer_index) {
     PSI_REQUIRE(ctx != nullptr, "ctx must not be null");
     Geometry g;
     int rc = make_geometry(cfg, &g);
@@ -151,8 +164,11 @@ extern "C" int psi_hip_kv_observe_weights(psi_hip_ctx* ctx, const psi_hip_gqa_co
     auto aligned = [](const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; };
     const bool two_byte = g.dtype == PSI_HIP_BF16 || g.dtype == PSI_HIP_F16;
     if (!ctx->force_generic && two_byte && (g.d == 128 || g.d == 256) && aligned(q) && aligned(kv_pages)) {
-        if (g.dtype == PSI_HIP_BF16) launch_observe_bf16(ctx, a);
-        else launch_observe_f16(ctx, a);
+        // not told: as many as there can be, if every window has one at least
+        const uint32_t most = num_rows > num_windows ? num_rows - num_windows + 1 : 1;
+        const uint32_t window_rows = max_window_rows != 0 ? max_window_rows : most;
+        if (g.dtype == PSI_HIP_BF16) launch_observe_bf16(ctx, a, window_rows);
+        else launch_observe_f16(ctx, a, window_rows);
         PSI_HIP_CHECK(hipGetLastError());
         return PSI_HIP_OK;
     }

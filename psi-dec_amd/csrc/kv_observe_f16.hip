@@ -2,5 +2,7 @@
 #include "kv_observe_kernel.h"
 
 namespace psi {
-void launch_observe_f16(psi_hip_ctx* ctx, const ObserveArgs& a) { launch_observe<F16Tag>(ctx, a); }
+void launch_observe_f16(psi_hip_ctx* ctx, const ObserveArgs& a, uint32_t window_rows) {
+    launch_observe<F16Tag>(ctx, a, window_rows);
+}
 }  // namespace psi

@@ -21,9 +21,11 @@
 
 namespace psi {
 
-// Normalisers are joined inside the second pass as long as (rows of a window) * (columns) stays within this, which saves
-// a launch (at 104: 13.2 for 15.7 us in all, at 1460: 59 for 62, at 6656: 10.9 for 13.3); at 10240 the two come out even,
-// and at 30016 (55 us in all) repeating the join in every workgroup costs 4 us.
+// Normalisers are joined inside the second pass as long as (rows of the longest window) * (columns) stays within this,
+// which saves a launch (at 104: 13.2 for 15.7 us in all, at 2496: 55.7 for 58.5, at 6656: 10.9 for 13.3); at 8064 and 9024
+// the two come out even (24.8 for 23.9, 59.2 for 58.8), and beyond, repeating the join in every workgroup of a long window
+// costs more than a launch, however short the other windows are (one prompt of 60000 beside three of 500, 22656: 44 for 39
+// us; one of 100000 beside 31 of 64, 57344: 53 for 44; one of 200000 beside 63 of 64, 94208: 139 for 117).
 constexpr uint64_t kFusedJoins = 8192;
 
 // Blocks of columns from which the waves of a short row share them: 64 tokens, 40 heads over 8, of one prompt of 1500
@@ -314,10 +316,10 @@ struct ObservePass {
     static constexpr int kTiles = kTiles_, kBlocks = kBlocks_, kWaves = kWaves_;
 };
 template <typename Tag, int D, int kMaxBlocks, typename Stats, typename Sum>
-inline void launch_observe_blocks(psi_hip_ctx* ctx, const ObserveArgs& a) {
+inline void launch_observe_blocks(psi_hip_ctx* ctx, const ObserveArgs& a, uint32_t window_rows) {
     const dim3 grid(a.num_rows * a.v.hkv);
     ObserveArgs fused = a;
-    const uint64_t joins = (uint64_t)a.num_rows / a.num_windows * a.max_window * a.group;
+    const uint64_t joins = (uint64_t)window_rows * a.max_window * a.group;
     if (joins <= kFusedJoins) fused.norm = nullptr;
     hipLaunchKernelGGL((observe_kernel<Tag, D, Stats::kTiles, Stats::kBlocks, kMaxBlocks, Stats::kWaves, false>), grid,
                        dim3(64 * Stats::kWaves), 0, ctx->stream, a);
@@ -326,20 +328,20 @@ inline void launch_observe_blocks(psi_hip_ctx* ctx, const ObserveArgs& a) {
                        dim3(64 * Sum::kWaves), 0, ctx->stream, fused);
 }
 template <typename Tag>
-inline void launch_observe(psi_hip_ctx* ctx, const ObserveArgs& a) {
+inline void launch_observe(psi_hip_ctx* ctx, const ObserveArgs& a, uint32_t window_rows) {
     // few columns: a fraction of the LDS, which launches faster (8 tokens over a prompt of 777: 13.3 for 14.2 us)
     const bool narrow = (uint64_t)a.max_window * a.group <= 64;
     if (a.v.d == 256) {
         using Pass = ObservePass<2, 2, 12>;
-        if (narrow) launch_observe_blocks<Tag, 256, 4, Pass, Pass>(ctx, a);
-        else launch_observe_blocks<Tag, 256, 16, Pass, Pass>(ctx, a);
+        if (narrow) launch_observe_blocks<Tag, 256, 4, Pass, Pass>(ctx, a, window_rows);
+        else launch_observe_blocks<Tag, 256, 16, Pass, Pass>(ctx, a, window_rows);
     } else {
         // 64 keys a turn for the maxima (with streaming loads 68 us; 78 with 32), 32 for the weights, whose sums need
         // registers too (57; 58 with 48)
         using Stats = ObservePass<4, 1, 12>;
         using Sum = ObservePass<2, 2, 12>;
-        if (narrow) launch_observe_blocks<Tag, 128, 4, Sum, Sum>(ctx, a);
-        else launch_observe_blocks<Tag, 128, 24, Stats, Sum>(ctx, a);
+        if (narrow) launch_observe_blocks<Tag, 128, 4, Sum, Sum>(ctx, a, window_rows);
+        else launch_observe_blocks<Tag, 128, 24, Stats, Sum>(ctx, a, window_rows);
     }
 }
 

@@ -77,6 +77,7 @@ class GQAKVObservePlan:
     num_q_tokens: int
     max_window: int
     scratch: object
+    max_window_rows: int = 0  # rows of the window that has most; 0: not known
 
 
 class GQAKVObserveKernels:
@@ -105,8 +106,9 @@ class GQAKVObserveKernels:
         table = _upload(self.device, words[:8 * len(rs) + 3 * n.value])
         with torch.cuda.stream(self.device.stream):
             buffer = torch.empty(scratch.value, dtype=torch.uint8, device=self.device.torch_device)
+        bounds = words[:8 * len(rs)].reshape(-1, 8)
         return GQAKVObservePlan(table[:8 * len(rs)], table[8 * len(rs):], len(rs), n.value, int(cu[-1]), most.value,
-                                buffer)
+                                buffer, int((bounds[:, 6] - bounds[:, 5]).max()))
 
     def invoke(self, plan: GQAKVObservePlan, q, kv_pages, page_ids, page_weights, page_table_index: int,
                decay: float = 1.0):
@@ -120,11 +122,11 @@ class GQAKVObserveKernels:
             raise ValueError("kv_pages: a contiguous arena of the configured type on the kernels' device is wanted")
         if plan.scratch.device != self.device.torch_device:
             raise ValueError("plan: one prepared on the kernels' device is wanted")
-        L.check(self.device.lib.psi_hip_kv_observe_weights(
+        L.check(self.device.lib.psi_hip_kv_observe_weights_rows(
             self.device.ctx, ctypes.byref(self._cfg), ctypes.byref(self._layout), _ptr(q), plan.num_q_tokens,
             _ptr(kv_pages), _nbytes(kv_pages), _ptr(page_ids), _ptr(plan.windows), plan.num_windows, plan.max_window,
-            _ptr(plan.rows), plan.num_rows, _ptr(plan.scratch), _nbytes(plan.scratch), _ptr(page_weights),
-            _nbytes(page_weights), decay, page_table_index))
+            _ptr(plan.rows), plan.num_rows, plan.max_window_rows, _ptr(plan.scratch), _nbytes(plan.scratch),
+            _ptr(page_weights), _nbytes(page_weights), decay, page_table_index))
 
 
 @dataclass
