@@ -17,6 +17,7 @@
 
 #include "common.h"
 #include "device_types.h"
+#include "kv_eviction.h"
 
 // Partial-state storage for callers that cannot allocate: one array per GPU, inside the library's code object,
 // held from the moment the library is loaded on that GPU until the process ends.  In host code `scratch` is only
@@ -130,6 +131,11 @@ int record_layer(psi_hip_ctx* ctx, const psi_hip_gqa_layer_config* cfg, const ps
     const uint32_t layer = in->gqa_layer_index;
     PSI_REQUIRE(!tiled || weights == nullptr,
                 "attention weights are accumulated by the SingleQ variant: prepare the batch with it");
+    if (weights != nullptr) {  // ahead of the launch that appends: a refused step leaves the cache as it was
+        CacheView view;
+        rc = check_kv_weights(acfg, layout, in->page_ids, layer, in->kv_pages_bytes, weights, s.num_total_tokens, &view);
+        if (rc != PSI_HIP_OK) return rc;
+    }
 
     const void* q = in->q;
     psi_hip_output_gate gate_storage;

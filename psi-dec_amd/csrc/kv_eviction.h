@@ -58,8 +58,12 @@ constexpr uint32_t kWindowWords = 8;
 // Fills the view; refuses accumulators that hold no page.  kv_pages_bytes 0: the arena's end is not checked.
 int make_cache_view(const Geometry& g, const psi_hip_page_table_layout* layout, const uint32_t* page_ids,
                     uint32_t gqa_layer_index, uint64_t kv_pages_bytes, uint64_t page_weights_bytes, CacheView* view);
-// The checks every one of these entry points makes of its request table's host values.
+// Refuses a context with device-side counts bound: these entry points take theirs by value.
 int check_no_replay_counts(const psi_hip_ctx* ctx);
+// What a step that accumulates asks of its weights (kv_weights.hip), so that a layer can ask it before its first launch.
+int check_kv_weights(const psi_hip_gqa_config* cfg, const psi_hip_page_table_layout* layout, const uint32_t* page_ids,
+                     uint32_t gqa_layer_index, uint64_t kv_pages_bytes, const psi_hip_kv_weights* weights,
+                     uint32_t num_total_tokens, CacheView* view);
 
 // Launches go to the context's GPU whatever the calling thread's current device is.
 class DeviceGuard {

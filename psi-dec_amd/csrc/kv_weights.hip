@@ -220,6 +220,24 @@ __global__ __launch_bounds__(kFinishThreads) void accumulate_kernel(WeightsArgs 
 
 static uint64_t logits_stride(uint32_t max_context_tokens) { return ((uint64_t)max_context_tokens + 63) / 64 * 64; }
 
+int check_kv_weights(const psi_hip_gqa_config* cfg, const psi_hip_page_table_layout* layout, const uint32_t* page_ids,
+                     uint32_t gqa_layer_index, uint64_t kv_pages_bytes, const psi_hip_kv_weights* weights,
+                     uint32_t num_total_tokens, CacheView* view) {
+    Geometry g;
+    int rc = make_geometry(cfg, &g);
+    if (rc != PSI_HIP_OK) return rc;
+    PSI_REQUIRE(weights->page_weights && weights->logits, "weight accumulation buffers must not be null");
+    PSI_REQUIRE(weights->decay >= 0.0f && weights->decay <= 1.0f, "the decay must lie in [0, 1]");
+    PSI_REQUIRE(num_total_tokens > 0 && weights->max_context_tokens > 0, "logits need tokens and a context");
+    PSI_REQUIRE(reinterpret_cast<uintptr_t>(weights->logits) % 16 == 0, "the logits must be 16-byte aligned");
+    uint64_t needed = 0;
+    rc = psi_hip_split_kv_single_q_logits_bytes(cfg, num_total_tokens, weights->max_context_tokens, &needed);
+    if (rc != PSI_HIP_OK) return rc;
+    PSI_REQUIRE(weights->logits_bytes >= needed, "logits buffer too small: %llu < %llu",
+                (unsigned long long)weights->logits_bytes, (unsigned long long)needed);
+    return make_cache_view(g, layout, page_ids, gqa_layer_index, kv_pages_bytes, weights->page_weights_bytes, view);
+}
+
 }  // namespace psi
 
 using namespace psi;
@@ -249,22 +267,13 @@ extern "C" int psi_hip_split_kv_single_q_attend_weights(
     if (rc != PSI_HIP_OK) return rc;
     PSI_REQUIRE((worker_cu == nullptr) == (num_workers == 0), "a worker table needs its worker count and vice versa");
     PSI_REQUIRE((flat_k == nullptr) == (flat_v == nullptr), "GQA KV page write needs K and V rows or neither");
-    PSI_REQUIRE(flat_token_indices && weights->page_weights && weights->logits && cu_kv_splits && output,
-                "weight accumulation buffers must not be null");
-    PSI_REQUIRE(weights->decay >= 0.0f && weights->decay <= 1.0f, "the decay must lie in [0, 1]");
-    PSI_REQUIRE(num_total_tokens > 0 && weights->max_context_tokens > 0, "logits need tokens and a context");
-    PSI_REQUIRE(reinterpret_cast<uintptr_t>(weights->logits) % 16 == 0, "the logits must be 16-byte aligned");
-    uint64_t needed = 0;
-    rc = psi_hip_split_kv_single_q_logits_bytes(cfg, num_total_tokens, weights->max_context_tokens, &needed);
-    if (rc != PSI_HIP_OK) return rc;
-    PSI_REQUIRE(weights->logits_bytes >= needed, "logits buffer too small: %llu < %llu",
-                (unsigned long long)weights->logits_bytes, (unsigned long long)needed);
+    PSI_REQUIRE(flat_token_indices && cu_kv_splits && output, "weight accumulation buffers must not be null");
     WeightsArgs a;
     ReduceArgs r;
+    rc = check_kv_weights(cfg, layout, page_ids, gqa_layer_index, kv_pages_bytes, weights, num_total_tokens, &a.v);
+    if (rc != PSI_HIP_OK) return rc;
     rc = single_q_reduce_args(ctx, cfg, scratch, scratch_bytes, cu_kv_splits, output, num_total_tokens,
                               num_total_kv_splits, num_active_tokens, partial_row_index, gate, &g, &r);
-    if (rc != PSI_HIP_OK) return rc;
-    rc = make_cache_view(g, layout, page_ids, gqa_layer_index, kv_pages_bytes, weights->page_weights_bytes, &a.v);
     if (rc != PSI_HIP_OK) return rc;
     PSI_REQUIRE((uint64_t)num_total_kv_splits * g.hkv <= 0x7fffffffull, "too many KV splits");
     a.v.num_weight_pages = std::min(a.v.num_weight_pages, a.v.num_pages);  // no page beyond the arena either
