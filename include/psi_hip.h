@@ -813,8 +813,12 @@ int psi_hip_gqa_replay_cache_stats(const psi_hip_gqa_replay_cache* cache, uint32
  * projection form, which takes the cache position for the rotary position, is for requests that were never compacted.
  *
  * Accumulators: page_weights, device f32 [page][num_kv_heads][tokens_per_page], found through the same page IDs as K
- * and V (every layer's pages are its own, so one array serves all layers).  A step starts the accumulators of the
- * tokens it appends from zero, so a page taken from the allocator needs no clearing.  A page belongs to one request;
+ * and V (every layer's pages are its own, so one array serves all layers).  attend_weights starts the accumulators of
+ * the tokens that its step appends from zero, observe_weights those of positions from num_held on; a page that is filled
+ * in these two ways only needs no clearing.  Every other step (plain, TiledQ, replayed, mixed) appends tokens and leaves
+ * their accumulators as the page's last owner left them: observe such tokens with the first of them as num_held before
+ * the next accumulating step or selection, or clear the accumulators of pages when they are issued.  A page belongs to one
+ * request;
  * accumulators of page IDs beyond the arena or the accumulators are left out (PSI_HIP_DEVICE_ERR_CACHE_RANGE), and so are
  * the K and V lines of such pages in observe_weights and compact.  attend_weights reads and appends K and V as the plain
  * decode map does: request slots and page IDs have to be valid there.

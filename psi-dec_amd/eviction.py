@@ -39,7 +39,11 @@ class GQAKVEvictionConfig:
 
 
 def page_weights(device: Device, config, num_pages: int):
-    """Accumulators for an arena of `num_pages` pages, zeroed; `config` is any of the kernels' configs."""
+    """Accumulators for an arena of `num_pages` pages, zeroed; `config` is any of the kernels' configs.
+
+    Only a step that accumulates and an observation (from `num_held` on) start the accumulators of new tokens from zero.
+    Where other steps append too (prefill, verify), observe their tokens before the next accumulating step or selection,
+    or zero a page's accumulators when it is issued again."""
     import torch
 
     out, cfg = ctypes.c_uint64(), config.struct()
