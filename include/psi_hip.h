@@ -806,9 +806,11 @@ int psi_hip_gqa_replay_cache_stats(const psi_hip_gqa_replay_cache* cache, uint32
  *   observe_weights  the same weights for the last tokens of a prompt (no attention output): what a prompt is cut by;
  *   select_kept      the positions to keep: the first num_first, the last num_recent, then the heaviest;
  *   compact          moves the kept lines and accumulators to the front of the request's pages.
- * Afterwards a request holds `budget` cached tokens: pages behind them can go back to the allocator, its next token is
- * appended at position `budget` (token_index of the next step), and the attention entry points above serve it as they
- * are.  Keys stay rotated for the positions they were written at, so the rotary position of a new token counts on
+ * Afterwards a request holds `budget` cached tokens: its next token is appended at position `budget` (token_index of the
+ * next step), the attention entry points above serve it as they are, and the pages behind are not read any more.  A
+ * caller that owns the pages (psi_hip_id_allocator) can free those; psi_hip_decoder_blocks keeps all pages of its request
+ * until the request is released, whatever was cut, and counts the request's tokens: its token_index less the evicted
+ * tokens is the cache position.  Keys stay rotated for the positions they were written at, so the rotary position of a new token counts on
  * (psi_hip_rms_norm_rope with positions of its own, then the split-row form of the layer); the layer's fused
  * projection form, which takes the cache position for the rotary position, is for requests that were never compacted.
  *
@@ -816,12 +818,12 @@ int psi_hip_gqa_replay_cache_stats(const psi_hip_gqa_replay_cache* cache, uint32
  * and V (every layer's pages are its own, so one array serves all layers).  attend_weights starts the accumulators of
  * the tokens that its step appends from zero, observe_weights those of positions from num_held on; a page that is filled
  * in these two ways only needs no clearing.  Every other step (plain, TiledQ, replayed, mixed) appends tokens and leaves
- * their accumulators as the page's last owner left them: observe such tokens with the first of them as num_held before
- * the next accumulating step or selection, or clear the accumulators of pages when they are issued.  A page belongs to one
- * request;
- * accumulators of page IDs beyond the arena or the accumulators are left out (PSI_HIP_DEVICE_ERR_CACHE_RANGE), and so are
- * the K and V lines of such pages in observe_weights and compact.  attend_weights reads and appends K and V as the plain
- * decode map does: request slots and page IDs have to be valid there.
+ * their accumulators as the place's last token left them: observe such tokens with the first of them as num_held before
+ * the next accumulating step or selection, or clear the places that they will fill (pages when they are issued, after a
+ * compaction also the places from `budget` on).  A page belongs to one request; accumulators of page IDs beyond the arena
+ * or the accumulators are left out (PSI_HIP_DEVICE_ERR_CACHE_RANGE), and so are the K and V lines of such pages in
+ * observe_weights and compact.  attend_weights reads and appends K and V as the plain decode map does: request slots and
+ * page IDs have to be valid there.
  * Weights, normalisers and sums are f32 whatever the cache's type.  Nothing is added atomically: the same call gives
  * the same bits on every run.  These entry points allocate nothing and can be captured into a graph; two launches of
  * one scratch, logits or kept buffer must follow one another. */

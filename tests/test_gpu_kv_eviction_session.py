@@ -1,14 +1,19 @@
-"""Eviction next to what else touches a cache: steps that append without accumulating."""
+"""Eviction next to what else touches a cache: steps that append without accumulating, the page-ID allocator, the page table
+and the block bookkeeping."""
+import importlib
+import types
+
 import numpy as np
 import pytest
 
-from eviction_util import attention_weights, page_rows
+from eviction_util import attention_weights, compacted, kept_positions, page_rows
 from parity_util import assert_outputs_close, importlib_workloads, oracle_step
 from test_gpu_kv_eviction import LAYERS, _assert_weights, _config
 
 pytestmark = pytest.mark.gpu
 
 HQ, HKV, D, PAGE = 8, 2, 128, 16
+runtime = importlib.import_module("psi-dec_amd.runtime")
 
 
 def _step(psi, w, seed, contexts, q_lens, requests=None):
@@ -92,3 +97,149 @@ def test_tokens_that_a_plain_step_appended(psi, oracle, device, route):
         cached = cached + q_lens
     got = acc.cpu().numpy()
     assert np.isfinite(got[_used(s, got.shape)]).all()
+
+
+def _cache(psi, device, slots, blocks, num_pages, seed):
+    """An arena of random bytes, its accumulators, a table of two layers, and what a step's workload needs of them."""
+    wl = importlib_workloads(psi)
+    layout = psi.GQAPageTableLayout(4, 2, blocks, 1)
+    table = psi.GQARequestPageTable(device, layout)
+    rng = np.random.default_rng(seed)
+    host = wl.to_storage(rng.standard_normal((num_pages, 2, HKV, PAGE, D)).astype(np.float32), psi.Dtype.Bfloat16)
+    c = types.SimpleNamespace(table=table, layout=layout, num_pages=num_pages, req_slots=np.asarray(slots, np.uint32),
+                              pages=host, layer=0, page_ids=None)
+    c.cfg = psi.GQAKVEvictionConfig(HQ, HKV, D, D ** -0.5, 2 * HKV * PAGE * D * 2, layout, psi.Dtype.Bfloat16)
+    c.d_pages = device.from_numpy(host.reshape(-1))
+    c.acc = psi.page_weights(device, c.cfg, num_pages).fill_(float("nan"))
+    return c
+
+
+def _view(c, device, layer):
+    device.sync()
+    c.layer, c.page_ids = layer, c.table.page_ids.cpu().numpy().view(np.uint32)
+    return c
+
+
+def _cut(psi, device, c, kernels, requests, cached):
+    """Selects and compacts both layers of some requests, next to the same on the host."""
+    plan = kernels.prepare(c.req_slots[requests], cached)
+    for layer in range(2):
+        _view(c, device, layer)
+        host_acc = c.acc.cpu().numpy()
+        kept = kernels.invoke_select(plan, c.acc, c.table.page_ids, layer)
+        kernels.invoke_compact(plan, kept, c.d_pages, c.acc, c.table.page_ids, layer)
+        for r, n in zip(requests, cached):
+            rows, p = page_rows(c, r), np.arange(n)
+            keep = [kept_positions(host_acc[rows[p // PAGE], h, p % PAGE], n, kernels.budget, kernels.num_first,
+                                   kernels.num_recent) for h in range(HKV)]
+            c.pages, host_acc = compacted(c.pages, host_acc, rows, keep, PAGE)
+        assert c.d_pages.cpu().numpy().tobytes() == c.pages.tobytes()
+        assert c.acc.cpu().numpy().tobytes() == host_acc.tobytes()
+
+
+def _prompt(psi, oracle, device, c, observe, requests, lens, seed):
+    """Prefill of whole prompts by plain steps, then their last eight tokens observe."""
+    for layer in range(2):
+        _view(c, device, layer)
+        s = _step(psi, c, seed + layer, lens, lens, requests)
+        out = _plain(psi, device, s, c.d_pages, c.table.page_ids)
+        c.pages, exp = oracle_step(oracle, s)
+        assert_outputs_close(out, exp, "prefill")
+        last = _step(psi, c, seed + layer, lens, [8] * len(lens), requests)
+        last.q = np.concatenate([s.q[int(s.cu_tokens[r + 1]) - 8:int(s.cu_tokens[r + 1])] for r in range(len(lens))])
+        before = c.acc.cpu().numpy()
+        plan = observe.prepare(last.req_slots, last.token_indices, last.cu_tokens, [0] * len(lens))
+        observe.invoke(plan, device.from_numpy(last.q.reshape(-1)), c.d_pages, c.table.page_ids, c.acc, layer)
+        _check_accumulators(last, c.pages, [0] * len(lens), 1.0, before, c.acc.cpu().numpy(), "prompt")
+
+
+def _decode(psi, oracle, device, c, requests, cached, seed):
+    for layer in range(2):
+        _view(c, device, layer)
+        s = _step(psi, c, seed + layer, np.asarray(cached) + 1, 1, requests)
+        before = c.acc.cpu().numpy()
+        out = _accumulating(psi, device, s, c.d_pages, c.table.page_ids, c.acc, 0.75)
+        c.pages, exp = oracle_step(oracle, s)
+        assert_outputs_close(out, exp, "decode")
+        _check_accumulators(s, c.pages, s.token_indices, 0.75, before, c.acc.cpu().numpy(), "decode")
+
+
+def test_freed_pages_go_to_another_request(psi, oracle, device):
+    """A cache that the caller's own table and the allocator hold: a prompt finds no pages until two requests are cut,
+    then gets theirs, with the accumulators they left there; all three decode and are cut again."""
+    alloc = runtime.U32IDAllocator(64)
+    c = _cache(psi, device, [2, 0, 3], 24, 64, 161)
+    owned = {}
+
+    def grow(r, tokens):
+        for layer in range(2):
+            mine = owned.setdefault((r, layer), [])
+            while len(mine) * PAGE < tokens:
+                mine.append(alloc.alloc_one())
+                c.table.write_page_ids(int(c.req_slots[r]), layer, len(mine) - 1, mine[-1:], c.num_pages)
+
+    def trim(r, tokens):
+        for layer in range(2):
+            keep = -(-tokens // PAGE)
+            alloc.free_many(owned[r, layer][keep:])
+            del owned[r, layer][keep:]
+
+    observe = psi.GQAKVObserveKernels(device, c.cfg)
+    evict = psi.GQAKVEvictionKernels(device, c.cfg, 60, 4, 16)
+    for r, n in ((0, 300), (1, 90)):
+        grow(r, n)
+    _prompt(psi, oracle, device, c, observe, [0, 1], [300, 90], 162)
+    assert alloc.free() == 14  # a prompt of 200 wants 26
+    before = set(owned[0, 0] + owned[0, 1] + owned[1, 0] + owned[1, 1])
+    _cut(psi, device, c, evict, [0, 1], [300, 90])
+    for r in (0, 1):
+        trim(r, 60)
+    grow(2, 200)
+    assert before & set(owned[2, 0] + owned[2, 1])
+    _prompt(psi, oracle, device, c, observe, [2], [200], 164)
+    _cut(psi, device, c, evict, [2], [200])
+    trim(2, 60)
+    cached = [60, 60, 60]
+    for step in range(12):
+        for r in range(3):
+            grow(r, cached[r] + 1)
+        _decode(psi, oracle, device, c, [0, 1, 2], cached, 170 + 2 * step)
+        cached = [n + 1 for n in cached]
+    _cut(psi, device, c, evict, [0, 1, 2], cached)
+    for r in range(3):
+        trim(r, 60)
+    assert alloc.used() == 3 * 2 * 4
+
+
+def test_a_request_of_the_block_bookkeeping(psi, oracle, device):
+    """DecoderBlocks counts the tokens of the request and owns its pages: the cut cache lives in the first of them, at
+    positions less by what was evicted, and all pages go back when the request does."""
+    alloc = runtime.U32IDAllocator(64)
+    c = _cache(psi, device, [1], 24, 64, 181)
+    blocks = runtime.DecoderBlocks(alloc, PAGE, 1, 2, range(91))
+
+    def schedule(tokens):
+        while blocks.ready_token_slots() < tokens:
+            assert blocks.init_block_once() != "ResourceLimitExceeded"
+        sync = blocks.prepare_blocks()
+        for i, ids in enumerate(sync.kv_page_ids[0]):
+            for layer in range(2):
+                c.table.write_page_ids(1, layer, sync.block_index + i, ids[layer:layer + 1], c.num_pages)
+        blocks.commit_blocks(sync)
+        return blocks.prepare(tokens)
+
+    query = schedule(90)
+    assert query.kind == "Prefill" and query.token_index == 0
+    observe = psi.GQAKVObserveKernels(device, c.cfg)
+    _prompt(psi, oracle, device, c, observe, [0], [90], 182)
+    blocks.commit(query, runtime.SampledTokens.prefill(query.epoch))
+    _cut(psi, device, c, psi.GQAKVEvictionKernels(device, c.cfg, 40, 4, 16), [0], [90])
+    evicted = 90 - 40
+    for step in range(20):
+        query = schedule(1)
+        assert query.kind == "Decode" and query.token_index == 90 + step
+        _decode(psi, oracle, device, c, [0], [query.token_index - evicted], 190 + 2 * step)
+        blocks.commit(query, runtime.SampledTokens.decode(query.epoch, [], 1000 + step))
+    assert len(blocks.cached_tokens()) == 110 and alloc.used() == 2 * 7
+    blocks.close()
+    assert alloc.used() == 0
