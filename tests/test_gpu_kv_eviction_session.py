@@ -1,12 +1,12 @@
 """Eviction next to what else touches a cache: steps that append without accumulating, the page-ID allocator, the page table
-and the block bookkeeping."""
+and the block bookkeeping, and rotary positions that count on behind a compaction."""
 import importlib
 import types
 
 import numpy as np
 import pytest
 
-from eviction_util import attention_weights, compacted, kept_positions, page_rows
+from eviction_util import attention_weights, compacted, kept_positions, page_rows, softmax_rows, to_f64
 from parity_util import assert_outputs_close, importlib_workloads, oracle_step
 from test_gpu_kv_eviction import LAYERS, _assert_weights, _config
 
@@ -243,3 +243,76 @@ def test_a_request_of_the_block_bookkeeping(psi, oracle, device):
     assert len(blocks.cached_tokens()) == 110 and alloc.used() == 2 * 7
     blocks.close()
     assert alloc.used() == 0
+
+
+def test_rotary_positions_count_on_behind_a_compaction(psi, device):
+    """Tokens are rotated for the position they have in the text and cached where the cut cache ends, through the layer's
+    split-row form; the plain cache is a list of rotated lines per head."""
+    import torch
+
+    wl = importlib_workloads(psi)
+    c = _cache(psi, device, [2], 24, 24, 201)
+    dev, dtype = device.torch_device, torch.bfloat16
+    for block in range(12):
+        for layer in range(2):
+            c.table.write_page_ids(2, layer, block, [2 * block + layer], 24)
+    layer, n, budget = 1, 120, 48
+    core = psi.GQACore(0, HQ * D, D, HQ, HKV, D ** -0.5)
+    gqa = psi.GQA.new(device, core, psi.GQAMetalConfig(c.cfg.page_bytes, 64, 1e-6, 1e4), False)
+    rope = {h: psi.RMSNormRopeKernel(device, psi.RMSNormRopeConfig(h, D, 64, 1e-6, 1e4)) for h in (HQ, HKV)}
+    gen = torch.Generator(device=dev).manual_seed(202)
+    norm = {h: torch.rand(D, generator=gen, device=dev).add_(0.5).to(dtype) for h in (HQ, HKV)}
+
+    def rotated(heads, rows, positions):
+        x = torch.randn(rows, heads, D, generator=gen, device=dev).to(dtype)
+        out = torch.empty_like(x)
+        rope[heads].invoke(rows, x, norm[heads], torch.as_tensor(positions, dtype=torch.int32, device=dev), out)
+        return x, out
+
+    def record(first, rows, text_first, weights=None):
+        meta = psi.GQAMetadataBuffers(device, rows, max_kv_splits=4 * rows)
+        shape = gqa.prepare_fixed_partition(meta, [2], [first], [0, rows], 64,
+                                            variant=psi.GQASplitKVVariant.SingleQ(16, 256, 4))
+        text = list(range(text_first, text_first + rows))
+        (_, q), (k_raw, k) = rotated(HQ, rows, text), rotated(HKV, rows, text)
+        if text_first != first:  # (the cache position would rotate otherwise)
+            other = torch.empty_like(k)
+            rope[HKV].invoke(rows, k_raw, norm[HKV], torch.arange(first, first + rows, dtype=torch.int32, device=dev), other)
+            assert not torch.equal(other, k)
+        v = torch.randn(rows, HKV, D, generator=gen, device=dev).to(dtype)
+        scratch = gqa.new_scratch(rows, shape.num_total_sdpa_map_task_templates)
+        inp = psi.GQAInput(c.layout, layer, meta, psi.GQAKVCacheBindings(c.d_pages, c.table.page_ids), scratch, q=q, k=k, v=v)
+        inp.output = torch.zeros(rows * HQ * D, device=dev)
+        inp.kv_weights = weights
+        device.f32_output(True)
+        gqa.record(inp)
+        device.f32_output(False)
+        device.sync()
+        return [t.view(torch.int16).cpu().numpy().view(np.uint16) for t in (q, k, v)] + [inp.output.cpu().numpy()]
+
+    q, k, v, _ = record(0, n, 0)
+    lines = [np.stack([k[:, h], v[:, h]], axis=1) for h in range(HKV)]  # [token][K, V][dim]
+    observe = psi.GQAKVObserveKernels(device, c.cfg)
+    observe.invoke(observe.prepare([2], [n - 16], [0, 16], [0]), device.from_numpy(q[-16:]), c.d_pages, c.table.page_ids,
+                   c.acc, layer)
+    evict = psi.GQAKVEvictionKernels(device, c.cfg, budget, 4, 8)
+    plan = evict.prepare([2], [n])
+    kept = evict.invoke_select(plan, c.acc, c.table.page_ids, layer)
+    evict.invoke_compact(plan, kept, c.d_pages, c.acc, c.table.page_ids, layer)
+    lines = [x[kept[0, h].cpu().numpy()] for h, x in enumerate(lines)]
+    weights = psi.GQAKVWeights(c.acc, gqa.new_logits(1, 64))
+    for step in range(8):
+        q, k, v, out = record(budget + step, 1, n + step, weights)
+        lines = [np.concatenate([x, np.stack([k[:, h], v[:, h]], axis=1)]) for h, x in enumerate(lines)]
+        exp = np.zeros((HQ, D))
+        for g in range(HQ):
+            keys, values = (to_f64(lines[g // (HQ // HKV)][:, i], psi.Dtype.Bfloat16) for i in (0, 1))
+            exp[g] = softmax_rows((keys @ to_f64(q[0, g], psi.Dtype.Bfloat16))[None, :] * D ** -0.5)[0] @ values
+        assert_outputs_close(out, exp, f"step {step}")
+    _view(c, device, layer)
+    pages = c.d_pages.cpu().numpy().view(np.uint16).reshape(c.pages.shape)
+    rows, p = page_rows(c, 0), np.arange(budget + 8)
+    for h in range(HKV):
+        assert np.array_equal(pages[rows[p // PAGE], :, h, p % PAGE], lines[h])
+    acc = c.acc.cpu().numpy()[rows[p // PAGE], :, p % PAGE]
+    assert np.isfinite(acc).all() and (acc > 0).all()
