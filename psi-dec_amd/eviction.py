@@ -17,8 +17,7 @@ from typing import Optional, Sequence
 import numpy as np
 
 from . import _lib as L
-from .gqa import (Device, Dtype, GQAPageTableLayout, _cfg_struct, _check_page_weights, _is_stored, _nbytes,
-                  _ptr, _tokens_per_page)
+from .gqa import Device, Dtype, GQAPageTableLayout, _cfg_struct, _check_page_weights, _is_stored, _tokens_per_page
 
 
 @dataclass(frozen=True)
@@ -64,6 +63,15 @@ def _p(a):
     return a.ctypes.data_as(ctypes.POINTER(ctypes.c_uint32)) if a is not None else None
 
 
+# What a launch call passes is made with as little as can be: the smallest launches take less time than ten conversions.
+def _addr(t):
+    return t.data_ptr() if t is not None else None
+
+
+def _size(t):
+    return t.nbytes if t is not None else 0
+
+
 def _upload(device: Device, array: np.ndarray):
     import torch
 
@@ -89,6 +97,8 @@ class GQAKVObserveKernels:
         config.num_tokens_per_page()  # validates
         self.device, self.config = device, config
         self._cfg, self._layout = config.struct(), config.page_table_layout.struct()
+        self._refs = ctypes.byref(self._cfg), ctypes.byref(self._layout)
+        self._torch_dtype = config.dtype.torch()
 
     def prepare(self, req_slots: Sequence[int], token_indices: Sequence[int], cu_tokens: Sequence[int],
                 num_held: Optional[Sequence[int]] = None) -> GQAKVObservePlan:
@@ -119,18 +129,17 @@ class GQAKVObserveKernels:
         """Adds the windows' weights to `page_weights`; `q`: [query tokens][Q heads][head_dim], rotated."""
         _check_page_weights(page_weights, self.device)
         if (q.numel() < plan.num_q_tokens * self.config.num_q_heads * self.config.head_dim or
-                q.element_size() != self.config.dtype.item_size() or not _is_stored(q, self.config.dtype, self.device)):
+                q.element_size() != self.config.dtype.item_size() or not _is_stored(q, self._torch_dtype, self.device)):
             raise ValueError("q: contiguous rows of the cache's type on the kernels' device are wanted, one for every "
                              "planned query token")
-        if not _is_stored(kv_pages, self.config.dtype, self.device):
+        if not _is_stored(kv_pages, self._torch_dtype, self.device):
             raise ValueError("kv_pages: a contiguous arena of the configured type on the kernels' device is wanted")
         if plan.scratch.device != self.device.torch_device:
             raise ValueError("plan: one prepared on the kernels' device is wanted")
         L.check(self.device.lib.psi_hip_kv_observe_weights_rows(
-            self.device.ctx, ctypes.byref(self._cfg), ctypes.byref(self._layout), _ptr(q), plan.num_q_tokens,
-            _ptr(kv_pages), _nbytes(kv_pages), _ptr(page_ids), _ptr(plan.windows), plan.num_windows, plan.max_window,
-            _ptr(plan.rows), plan.num_rows, plan.max_window_rows, _ptr(plan.scratch), _nbytes(plan.scratch),
-            _ptr(page_weights), _nbytes(page_weights), decay, page_table_index))
+            self.device.ctx, *self._refs, _addr(q), plan.num_q_tokens, _addr(kv_pages), _size(kv_pages), _addr(page_ids),
+            _addr(plan.windows), plan.num_windows, plan.max_window, _addr(plan.rows), plan.num_rows, plan.max_window_rows,
+            _addr(plan.scratch), _size(plan.scratch), _addr(page_weights), _size(page_weights), decay, page_table_index))
 
 
 @dataclass
@@ -156,6 +165,8 @@ class GQAKVEvictionKernels:
         self.device, self.config = device, config
         self.budget, self.num_first, self.num_recent = budget, num_first, num_recent
         self._cfg, self._layout = config.struct(), config.page_table_layout.struct()
+        self._refs = ctypes.byref(self._cfg), ctypes.byref(self._layout)
+        self._torch_dtype = config.dtype.torch()
 
     def prepare(self, req_slots: Sequence[int], num_cached: Sequence[int]) -> GQAKVEvictionPlan:
         """`num_cached[r]`: the tokens that request r's cache holds.  psi_hip_kv_evict_plan and one upload."""
@@ -179,8 +190,8 @@ class GQAKVEvictionKernels:
 
     def _check_plan(self, plan: GQAKVEvictionPlan):
         """A plan has room for what its own kernels keep: another budget or head count would leave it."""
-        wanted = (plan.num_reqs, self.config.num_kv_heads, self.budget)
-        if tuple(plan.kept.shape) != wanted or plan.kept.device != self.device.torch_device:
+        kept, wanted = plan.kept, (plan.num_reqs, self.config.num_kv_heads, self.budget)
+        if kept.shape != wanted or kept.device != self.device.torch_device:
             raise ValueError(f"plan: one prepared by kernels of this budget, head count and device is wanted; it keeps "
                              f"{tuple(plan.kept.shape)} positions on {plan.kept.device}, these kernels {wanted}")
 
@@ -191,24 +202,22 @@ class GQAKVEvictionKernels:
         self._check_plan(plan)
         _check_page_weights(page_weights, self.device)
         L.check(self.device.lib.psi_hip_kv_select_kept(
-            self.device.ctx, ctypes.byref(self._cfg), ctypes.byref(self._layout), _ptr(page_weights),
-            _nbytes(page_weights), _ptr(page_ids), _ptr(plan.requests), plan.num_reqs, plan.max_cached, self.budget,
-            self.num_first, self.num_recent, _ptr(plan.kept), _ptr(plan.scratch), _nbytes(plan.scratch), page_table_index))
+            self.device.ctx, *self._refs, _addr(page_weights), _size(page_weights), _addr(page_ids), _addr(plan.requests),
+            plan.num_reqs, plan.max_cached, self.budget, self.num_first, self.num_recent, _addr(plan.kept),
+            _addr(plan.scratch), _size(plan.scratch), page_table_index))
         return plan.kept
 
     def invoke_compact(self, plan: GQAKVEvictionPlan, kept, kv_pages, page_weights, page_ids, page_table_index: int):
         """Moves the kept lines of `kv_pages` and their accumulators (`page_weights` may be None) to the front."""
-        import torch
-
         self._check_plan(plan)
         if page_weights is not None:
             _check_page_weights(page_weights, self.device)
-        if (kept.dtype != torch.int32 or not kept.is_contiguous() or kept.numel() != plan.kept.numel() or
-                kept.device != self.device.torch_device):
+        if kept is not plan.kept and (kept.dtype != plan.kept.dtype or not kept.is_contiguous() or
+                                      kept.numel() != plan.kept.numel() or kept.device != self.device.torch_device):
             raise ValueError("kept: the contiguous int32 [requests][KV heads][budget] of a selection is wanted")
-        if not _is_stored(kv_pages, self.config.dtype, self.device):
+        if not _is_stored(kv_pages, self._torch_dtype, self.device):
             raise ValueError("kv_pages: a contiguous arena of the configured type on the kernels' device is wanted")
         L.check(self.device.lib.psi_hip_kv_compact(
-            self.device.ctx, ctypes.byref(self._cfg), ctypes.byref(self._layout), _ptr(kv_pages), _nbytes(kv_pages),
-            _ptr(page_weights), _nbytes(page_weights), _ptr(page_ids), _ptr(plan.requests), plan.num_reqs,
-            plan.max_cached, self.budget, _ptr(kept), page_table_index))
+            self.device.ctx, *self._refs, _addr(kv_pages), _size(kv_pages), _addr(page_weights), _size(page_weights),
+            _addr(page_ids), _addr(plan.requests), plan.num_reqs, plan.max_cached, self.budget, _addr(kept),
+            page_table_index))

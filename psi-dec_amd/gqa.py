@@ -1034,9 +1034,9 @@ def _check_page_weights(weights, device: Device):
         raise ValueError("page_weights: a contiguous float32 tensor on the kernels' device is wanted")
 
 
-def _is_stored(t, dtype: Dtype, device: Device) -> bool:
-    """Contiguous storage of `dtype` on the kernels' device; integers are taken as its bytes."""
-    of_type = t.dtype == dtype.torch() or not (t.is_floating_point() or t.is_complex())
+def _is_stored(t, torch_dtype, device: Device) -> bool:
+    """Contiguous storage of a type on the kernels' device; integers are taken as its bytes."""
+    of_type = t.dtype == torch_dtype or not (t.is_floating_point() or t.is_complex())
     return of_type and t.is_contiguous() and t.device == device.torch_device
 
 
