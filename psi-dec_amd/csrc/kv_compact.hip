@@ -246,8 +246,8 @@ __global__ __launch_bounds__(kLevelThreads) void compact_level_kernel(CompactArg
 }
 
 // Slices of a line: down to 128 bytes until there are four workgroups to a compute unit (32 requests of 1k-8k tokens cut
-// to 1024, 4 heads of 256: 86 us with whole lines, 48 us with 128 bytes, which is 5.4 TB/s read and written); where that
-// leaves compute units without one, down to 32 bytes (one request of 8000 cut to 4000, 2 heads of 256: 14.4 us, 15.3 with
+// to 1024, 4 heads of 256: 86 us with whole lines, 48 us with 128 bytes, both with part of the lines in the memory-side
+// cache; with none there 57 us, which is 4.6 TB/s read and written); where that leaves compute units without one, down to 32 bytes (one request of 8000 cut to 4000, 2 heads of 256: 14.4 us, 15.3 with
 // 64 bytes; two of 65536 cut to 50000, 4 heads of 128: 164 and 172 us).
 inline uint32_t compact_slices(uint64_t pairs, uint32_t line_bytes) {
     uint32_t slices = 1;
@@ -272,8 +272,9 @@ inline uint32_t compact_levels(uint64_t groups, uint32_t budget, uint32_t max_ca
 
 template <typename Unit>
 static void launch_compact(psi_hip_ctx* ctx, const CompactArgs& a, uint32_t grid) {
-    // Many workgroups: a unit a lane, four workgroups to a compute unit, streaming loads (the 32 requests above: 48 us; 57
-    // with two units, whose registers leave room for three; 65 with ordinary loads, 65 with the other launch).  Few: long
+    // Many workgroups: a unit a lane, four workgroups to a compute unit, streaming loads (the 32 requests above, cached in
+    // part: 48 us; 57 with two units, whose registers leave room for three; 65 with ordinary loads, 65 with the other
+    // launch).  Few: long
     // runs and ordinary loads, as slices share lines of memory (one of 8000 cut to 4000: 14.4 us, 18.9 with the other
     // launch; four of 16000 cut to 8000: 61 and 76 us).
     if (grid >= 512)

@@ -13,7 +13,9 @@ __device__ __forceinline__ float dot_line(const ObserveArgs& a, uint64_t q_off, 
     return dot;
 }
 
-// Any head_dim, page size and type.  One wave per (row, query head); lane = key.
+// Any head_dim, page size and type.  One wave per (row, query head); lane = key.  Bound by the scalar products: 8 prompts of
+// 1k-8k, 32 tokens, 24 heads over 4, take 13 ms with bf16 and D 64, 47 ms with f32 and D 256 (the matrix-core kernels 0.06
+// ms with bf16 and D 256).
 template <typename Tag>
 __global__ __launch_bounds__(64) void observe_stats_generic(ObserveArgs a) {
     const uint32_t row = blockIdx.x / a.hq, head = blockIdx.x % a.hq, kv_head = head / a.group, lane = threadIdx.x;

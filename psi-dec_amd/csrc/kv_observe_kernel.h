@@ -11,9 +11,10 @@
 // lane and then over the four lanes of the column, the weights of a key (second pass) over the columns of a lane first
 // and over the lanes once per turn.  Where waves share the columns of a key, their sums meet in LDS.
 //
-// Measured: 8 prompts of 1k-8k (bf16, D 256, 32 tokens, 24 heads over 4) 58 us for two walks of 75 MB and 2 * 14 GFLOP;
-// one prompt of 65536 (D 128, 64 tokens, 40 heads over 8) 119 us for 2 * 134 MB and 2 * 43 GFLOP, 720 TFLOP/s.  The first
-// is bound by the lines: a workgroup has two turns, each a burst of reads and then a wait (27 of 33 us of its first pass
+// Measured: 8 prompts of 1k-8k (bf16, D 256, 32 tokens, 24 heads over 4) 56-61 us for two walks of 75 MB and 2 * 14
+// GFLOP; one prompt of 65536 (D 128, 64 tokens, 40 heads over 8) 122-126 us for 2 * 134 MB and 2 * 43 GFLOP, 690 TFLOP/s.
+// More columns than the LDS holds at a time (256 with D 256, 384 with D 128) take another walk over the keys for each
+// such part in both passes: a whole prompt of 2048 tokens 0.58 ms (40 heads over 8 of 128).  The first of these is bound by the lines: a workgroup has two turns, each a burst of reads and then a wait (27 of 33 us of its first pass
 // remained with a sixth of the products).  The second is bound by products and exponentials, which share a SIMD's issue.
 #pragma once
 #include "kv_observe.h"

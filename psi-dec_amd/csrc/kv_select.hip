@@ -99,8 +99,7 @@ struct BinSearch {
     uint32_t chosen[2];
 };
 // The counter that the `remaining`-th largest key falls into, and how many of that counter's keys are still to be kept.
-// Thread t brings the counts of the two highest counters it has not been beaten to: counters kBins - 1 - 2t and the one
-// below.  Returns the exclusive sum over the counters above the thread's in `above`.
+// Thread t brings the counts of counters kBins - 1 - 2t (`high`) and the one below (`low`).
 __device__ __forceinline__ void find_bin(BinSearch& lds, uint32_t tid, uint32_t high, uint32_t low, SelectState& st, int digit) {
     const uint32_t lane = tid & 63, wave = tid >> 6;
     uint32_t sum = high + low;

@@ -59,7 +59,7 @@ __device__ __forceinline__ float2 norm_of(const WeightsArgs& a, uint32_t p0, uin
 // where a page holds a multiple of four tokens, and a whole row in one turn if it has up to 2048 keys.
 // The chain of dependent reads is what bounds it (table row -> tokens -> partial states -> logits -> accumulators, each a
 // round trip), so the first turn's logits and page IDs are asked for before the normalisers are.  With the combine beside
-// it: 11.4 us for 25 MB at 32 requests of 1k-8k (the combine alone takes 6), 13.0 us for 49 MB (3.8 TB/s) at four of
+// it: 12.1 us for 25 MB at 32 requests of 1k-8k (the combine alone takes 6), 13.2 us for 49 MB (3.7 TB/s) at four of
 // 131072; two to four workgroups a row repeat the chain and take longer (an earlier form: 22 us for 15).
 __device__ __forceinline__ void accumulate_row(const WeightsArgs& a, uint32_t split, uint32_t kv_head, float2* norm) {
     const uint32_t num_tokens = active_count(a.replay_counts, kReplayTokens, a.num_active_tokens);

@@ -512,7 +512,8 @@ inline void launch_decode_map_w(psi_hip_ctx* ctx, const Geometry& g, const MapAr
     uint32_t lds = 0;
     if (kLogits) {
         // All of a compute unit's LDS if the launch has a workgroup per unit (a balanced plan), else half of it, so that
-        // a second workgroup streams while the first one starts or ends.
+        // a second workgroup streams while the first one starts or ends.  (With all of it, a workgroup of another stream
+        // that needs LDS waits for the unit until this one ends.)
         const uint32_t resident = grid.x <= (uint32_t)ctx->num_cus ? 1 : 2;
         const uint32_t tile = 4 * kTileTokens * G * 4;  // of the four waves
         a.logit_lds_tiles = (kLdsPerUnit / resident - decode_lds_bytes(D, G)) / tile;

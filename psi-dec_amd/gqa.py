@@ -1519,7 +1519,8 @@ class GQA:
     def record(self, inp: GQAInput):
         """`GQA::record` (backend.rs:394-658): issues the layer's launches on the device's stream and returns
         the output buffer (the reference returns the caller-owned buffer it was given, too).  With `inp.kv_weights`
-        the attention also accumulates its weights (psi_hip_gqa_layer_record_weights; not in the reference)."""
+        the attention also accumulates its weights (psi_hip_gqa_layer_record_weights; not in the reference).  Projection
+        output is rotated for the cache positions: a request whose cache was cut takes split rows, rotated by the caller."""
         cfg = self.struct()
         s, keep = self.input_struct(inp, takes_weights=True)
         if inp.kv_weights is not None:

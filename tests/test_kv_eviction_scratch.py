@@ -32,6 +32,18 @@ def test_scratch_never_falls_with_a_larger_capacity(psi, hkv):
             assert table[i, j] <= CHUNK_BYTES * max(large, 256)
 
 
+@pytest.mark.parametrize("hkv", [1, 3, 8, 300])
+def test_observation_scratch_has_a_bound_over_all_batches(psi, hkv):
+    from test_kv_eviction_host import _observe_plan
+
+    cfg, rng = _config(psi, hq=2 * hkv, hkv=hkv, d=8, slots=80, blocks=8192), np.random.default_rng(37)
+    for reqs in (1, 2, 7, 40, 80):
+        firsts, sizes = rng.integers(0, 120000, reqs), rng.integers(1, 65, reqs)
+        cu = np.concatenate([[0], np.cumsum(sizes)])
+        _, rows, most, scratch = _observe_plan(psi, cfg, range(reqs), firsts, cu)
+        assert scratch <= (max(256 // hkv, reqs, 1) * most + int(cu[-1])) * 2 * hkv * 8
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("hkv,large,small", [(8, [32768] * 5, [32768, 17001, 30000, 32768]),
                                              (2, [140000, 16], [131072]), (1, [600000], [524288])])
