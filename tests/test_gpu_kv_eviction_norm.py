@@ -36,3 +36,23 @@ def test_equal_keys_weigh_one_nth_each(psi, device, hq, hkv, d, dtype, lens):
     _, weights = _attend(psi, device, w, acc, 1.0)
     device.sync()
     _assert_equal_weights(w, weights)
+
+
+@pytest.mark.parametrize("hq,hkv,d,dtype", [(12, 2, 256, "Bfloat16"), (8, 1, 128, "Bfloat16"), (4, 2, 64, "Bfloat16")])
+@pytest.mark.parametrize("tokens", [1, 3])
+def test_a_step_over_keys_that_nothing_can_attend_to(psi, device, hq, hkv, d, dtype, tokens):
+    """Keys with an element of -inf under queries that are all positive: their weights are 0, and the others' sum to one
+    per query, also where a whole row of the plan holds such keys only."""
+    wl = importlib_workloads(psi)
+    w = wl.make_workload(122, [400, 30], hq, hkv, d, getattr(psi.Dtype, dtype), 16, q_lens=[tokens, 1], **LAYERS)
+    w.q = np.where((w.q & 0x7fff) == 0, 0x3f80, w.q & 0x7fff).astype(np.uint16)
+    rows, dead = page_rows(w, 0), np.r_[5, 64:128, 390]
+    w.pages[rows[dead // 16], 0, :, dead % 16, d - 1] = 0xff80
+    acc = np.full((w.num_pages, hkv, 16), 3.0, np.float32)
+    _, weights = _attend(psi, device, w, acc, 0.0, partition=64, balanced=False)
+    device.sync()
+    p, group = np.arange(400), hq // hkv
+    mine = weights.cpu().numpy()[rows[p // 16], :, p % 16]
+    assert np.isfinite(mine).all() and (mine[dead] == 0.0).all()
+    # 400 weights of a few queries, each a few roundings of exp2 and of a normaliser of 400 terms
+    assert np.abs(mine.sum(axis=0) / (tokens * group) - 1.0).max() <= HALF_ULP32 * (2 * 400 + tokens * group + 64)
