@@ -1036,6 +1036,8 @@ def _check_page_weights(weights, device: Device):
 
 def _is_stored(t, torch_dtype, device: Device) -> bool:
     """Contiguous storage of a type on the kernels' device; integers are taken as its bytes."""
+    if t is None:
+        return False
     of_type = t.dtype == torch_dtype or not (t.is_floating_point() or t.is_complex())
     return of_type and t.is_contiguous() and t.device == device.torch_device
 

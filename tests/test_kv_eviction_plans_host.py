@@ -112,3 +112,17 @@ def test_logits_on_another_device_are_refused(psi, host):
     logits = types.SimpleNamespace(buffer=torch.empty(64, device="meta"), bytes=256, max_context_tokens=64)
     with pytest.raises(ValueError, match="logits: room on the kernels' device"):
         psi.GQAKVWeights(_weights(host), logits).struct(host)
+
+
+def test_missing_pages_are_refused(psi, host):
+    import torch
+
+    ids = torch.zeros(1024, dtype=torch.int32)
+    observe = psi.GQAKVObserveKernels(host, _config(psi))
+    q = torch.zeros(4 * 24 * 256, dtype=torch.bfloat16)
+    with pytest.raises(ValueError, match="kv_pages: a contiguous"):
+        observe.invoke(observe.prepare([3], [100], [0, 4]), q, None, ids, _weights(host), 0)
+    evict = psi.GQAKVEvictionKernels(host, _config(psi), 32)
+    plan = evict.prepare([1], [100])
+    with pytest.raises(ValueError, match="kv_pages: a contiguous"):
+        evict.invoke_compact(plan, plan.kept, None, None, ids, 0)
